@@ -327,6 +327,142 @@ int kore_hip_pack_weights_ternary(const float *w, uint64_t m, uint64_t k,
                                   float threshold, uint8_t *packed,
                                   float *scales, kore_stream_t stream);
 
+/* ------------------------------------- query/key norm with rotation
+ * Per head row x of Q (weight q_weight[head_dim]) and K (k_weight[head_dim]),
+ * over its head_dim values: y = R(p) ((x * inv) * weight), inv = 1 /
+ * sqrt(sum x^2 / head_dim + eps), R(p) the rotation of kore_hip_rope_f32
+ * (interleaved as there) at the token's position p: positions[token] (a device
+ * array of batch * seq_len, read as unsigned) or, with positions NULL,
+ * start_pos + token % seq_len.  The angle p * inv_freq[i] is not rounded to
+ * f32, which kore_hip_rope_f32's is (as the reference's): the two differ by
+ * what that rounding is worth, 2^-24 of the angle.
+ * The reference composes RMSNorm (crates/kore-kernels/src/cpu_fused.rs:160-190)
+ * per head with apply_rope (crates/kore-edge/src/ops/rope.rs:9-36) and has no
+ * fused op.  f32 tol (sums are trees).
+ * Rows of a token are contiguous, [heads, head_dim]; tokens are a stride of
+ * floats apart (0: heads * head_dim), so q and k may be parts of one fused
+ * projection's output.  head_dim is even, at most 1024.  q_out may be q and
+ * k_out k (same stride); otherwise outputs overlap no input and not each other
+ * (KORE_HIP_ERR_ALIAS).  What lies between a token's rows is left as it is. */
+int kore_hip_qk_norm_rope_f32(const float *q, const float *k,
+                              const float *q_weight, const float *k_weight,
+                              const float *inv_freq, const uint32_t *positions,
+                              float *q_out, float *k_out, uint64_t batch,
+                              uint64_t seq_len, uint32_t q_heads,
+                              uint32_t k_heads, uint32_t head_dim,
+                              uint64_t q_stride, uint64_t k_stride,
+                              uint64_t q_out_stride, uint64_t k_out_stride,
+                              uint64_t start_pos, float eps, int interleaved,
+                              kore_stream_t stream);
+
+/* Its backward: from the gradients of q_out and k_out, with the inputs q and k
+ * of the forward, per row g = R(p)^T grad_out, n = x * inv, u = g * weight:
+ *   grad_x = inv * (u - n * mean(u * n)),   grad_weight = sum over rows g * n
+ * (grad_weight overwritten; summed over tokens and heads in a fixed order, so
+ * calls repeat bit for bit).  workspace: device scratch of at least
+ * kore_hip_qk_norm_rope_backward_workspace_bytes(batch * seq_len, ...) bytes
+ * (KORE_HIP_ERR_BAD_DIM if less); calls that may overlap in time need
+ * workspaces of their own.  grad_q may be grad_q_out or q, grad_k likewise
+ * (same stride); otherwise they overlap no input.  No tokens: the weight
+ * gradients are zeroed.  f32 tol. */
+uint64_t kore_hip_qk_norm_rope_backward_workspace_bytes(uint64_t tokens,
+                                                        uint32_t q_heads,
+                                                        uint32_t k_heads,
+                                                        uint32_t head_dim);
+
+int kore_hip_qk_norm_rope_backward_f32(
+    const float *grad_q_out, const float *grad_k_out, const float *q,
+    const float *k, const float *q_weight, const float *k_weight,
+    const float *inv_freq, const uint32_t *positions, float *grad_q,
+    float *grad_k, float *grad_q_weight, float *grad_k_weight,
+    float *workspace, uint64_t workspace_bytes, uint64_t batch,
+    uint64_t seq_len, uint32_t q_heads, uint32_t k_heads, uint32_t head_dim,
+    uint64_t grad_q_out_stride, uint64_t grad_k_out_stride, uint64_t q_stride,
+    uint64_t k_stride, uint64_t grad_q_stride, uint64_t grad_k_stride,
+    uint64_t start_pos, float eps, int interleaved, kore_stream_t stream);
+
+/* -------------------------------------------------- 4-bit key/value cache
+ * Keys and values of one layer in num_pages pages of page_size tokens, quantised
+ * as they are written.  Every 32 values of a head (zeros past head_dim) are a
+ * block: 32 E2M1 codes (sign, 2 exponent bits, 1 mantissa bit; magnitudes 0,
+ * 0.5, 1, 1.5, 2, 3, 4, 6) and a scale byte b that stands for 2^(b - 127), or
+ * for NaN if b = 255.  The scale is the smallest 2^e, -100 <= e <= 126, with
+ * which the block's largest magnitude is at most 7; a code is the nearest
+ * magnitude of x / 2^e, ties to the even code, 6 for all above 5 (at e = 126,
+ * magnitudes count as at most 3, so that nothing finite reads back infinite).
+ * A block with an infinity or a NaN reads back as 32 NaN.  Exact: the codes and
+ * scales are those of this definition.
+ * With nb = ceil(head_dim / 32) and P = page_size (a power of two, 16 to
+ * 65536), a page is kv_heads pieces, one after the other, of
+ *   [P][16 nb] K codes (dimension 2j in the low half of byte j),
+ *   [P/16][4][4 nb][4][4] V codes (token 4 g + i of 16 and dimensions 8c .. 8c+7
+ *     at [g][c][i]),  [P][nb] K scales,  [P/16][nb][16] V scales,
+ * P * nb * 34 bytes; kore_hip_kv_cache_q4_bytes is the whole size (0 for
+ * dimensions that are refused).  cache is 16-byte aligned; head_dim <= 256.
+ * The reference keeps its cache in f32 (crates/kore-attention/src/kv_cache.rs:11). */
+uint64_t kore_hip_kv_cache_q4_bytes(uint64_t num_pages, uint64_t page_size,
+                                    uint64_t kv_heads, uint64_t head_dim);
+
+/* Token t's K and V ([kv_heads, head_dim], tokens k_stride and v_stride floats
+ * apart, 0: kv_heads * head_dim) go to slot slots[t] = page * page_size + token
+ * of the page.  A slot past the last page (0xffffffff of a padded batch) is not
+ * written.  Nothing else in the cache changes.  A slot may appear once in a
+ * call: if it appears again, what it holds is a mix of its tokens' blocks. */
+int kore_hip_kv_cache_write_q4_f32(const float *k, const float *v,
+                                   const uint32_t *slots, uint8_t *cache,
+                                   uint64_t tokens, uint64_t kv_heads,
+                                   uint64_t head_dim, uint64_t num_pages,
+                                   uint64_t page_size, uint64_t k_stride,
+                                   uint64_t v_stride, kore_stream_t stream);
+
+/* The values that the cache holds for slots[t], as k_out and v_out[tokens,
+ * kv_heads, head_dim]; zeros for a slot past the last page.  Exact. */
+int kore_hip_kv_cache_read_q4_f32(const uint8_t *cache, const uint32_t *slots,
+                                  float *k_out, float *v_out, uint64_t tokens,
+                                  uint64_t kv_heads, uint64_t head_dim,
+                                  uint64_t num_pages, uint64_t page_size,
+                                  kore_stream_t stream);
+
+/* Attention over the 4-bit cache: for each sequence s and each of its query
+ * tokens, out = softmax(scale * q k^T) v over the sequence's first kv_lens[s]
+ * cached tokens, token i in page page_table[s][i / page_size] (max_pages
+ * entries a sequence).  Query heads h .. of group q_heads / kv_heads share key
+ * head h / group.  q[tokens, q_heads, head_dim] (tokens q_stride floats apart,
+ * 0: contiguous) holds the sequences' new tokens one after the other: those of
+ * s are q_starts[s] .. q_starts[s + 1] - 1 (num_seqs + 1 entries, ascending),
+ * any number of each, none included.  causal: the new tokens are the last ones
+ * of their sequence, and each sees the keys up to its own; otherwise all see
+ * all.  A row that sees no key is zeros.  Rows before q_starts[0] and from
+ * q_starts[num_seqs] on are not written.  Lengths past max_pages * page_size
+ * count as that, starts past `tokens` as that, and tokens of a page >= num_pages
+ * are left out.  Keys and values that a row does not see have no part in it, NaN
+ * included.
+ * The result is that of the cached values in f32 (f32 tol): products with the
+ * 4-bit values are exact, sums f32, probabilities 16 bits.
+ * The reference attends in f32 on the CPU (crates/kore-attention/src/flash.rs:28).
+ * workspace (16-byte aligned): kore_hip_attention_q4_workspace_bytes bytes,
+ * which may be 0; less is KORE_HIP_ERR_BAD_DIM.  Calls that may overlap in time
+ * need workspaces of their own.  out overlaps no input (KORE_HIP_ERR_ALIAS). */
+uint64_t kore_hip_attention_q4_workspace_bytes(uint64_t num_seqs,
+                                               uint64_t tokens,
+                                               uint64_t q_heads,
+                                               uint64_t kv_heads,
+                                               uint64_t head_dim,
+                                               uint64_t page_size,
+                                               uint64_t max_pages);
+
+int kore_hip_attention_q4_f32(const float *q, const uint8_t *cache,
+                              const uint32_t *page_table,
+                              const uint32_t *kv_lens,
+                              const uint32_t *q_starts, float *out,
+                              float *workspace, uint64_t workspace_bytes,
+                              uint64_t num_seqs, uint64_t tokens,
+                              uint64_t q_heads, uint64_t kv_heads,
+                              uint64_t head_dim, uint64_t num_pages,
+                              uint64_t page_size, uint64_t max_pages,
+                              uint64_t q_stride, float scale, int causal,
+                              kore_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -53,12 +53,22 @@ SIGNATURES = {
     "kore_hip_bit_linear_f32": [_ptr, _ptr, _ptr, _ptr, _ptr, _u64, _u64, _u64, _ptr],
     "kore_hip_bit_linear_i8": [_ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _u64, _u64, _u64, _ptr],
     "kore_hip_pack_weights_ternary": [_ptr, _u64, _u64, _f32, _ptr, _ptr, _ptr],
+    "kore_hip_qk_norm_rope_f32": [_ptr] * 8 + [_u64, _u64, _u32, _u32, _u32, _u64, _u64, _u64, _u64, _u64, _f32, _int,
+                                               _ptr],
+    "kore_hip_qk_norm_rope_backward_f32": [_ptr] * 13 + [_u64, _u64, _u64, _u32, _u32, _u32] + [_u64] * 7 +
+                                          [_f32, _int, _ptr],
+    "kore_hip_kv_cache_write_q4_f32": [_ptr] * 4 + [_u64] * 7 + [_ptr],
+    "kore_hip_kv_cache_read_q4_f32": [_ptr] * 4 + [_u64] * 5 + [_ptr],
+    "kore_hip_attention_q4_f32": [_ptr] * 7 + [_u64] * 10 + [_f32, _int, _ptr],
 }
 
 # Entry points whose return type is not int.
 RESTYPES = {
     "kore_hip_rms_norm_backward_workspace_bytes": ([_u64, _u64], _u64),
     "kore_hip_rms_norm_backward_noalloc_max_bytes": ([], _u64),
+    "kore_hip_qk_norm_rope_backward_workspace_bytes": ([_u64, _u32, _u32, _u32], _u64),
+    "kore_hip_kv_cache_q4_bytes": ([_u64] * 4, _u64),
+    "kore_hip_attention_q4_workspace_bytes": ([_u64] * 7, _u64),
 }
 
 

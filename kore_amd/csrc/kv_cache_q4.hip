@@ -1,0 +1,233 @@
+// kv_cache_q4.hip -- quantising keys and values into the paged 4-bit cache as
+// they are written, and reading tokens back.
+//
+// Scale of a block: the smallest 2^e, e in [-100, 126], with amax <= 7 * 2^e.
+// With amax in (3.5, 7] units the largest value is at most one unit from its
+// code (6 for everything above 5): no more than the widest step (4 to 6)
+// rounds anyway, so nothing is lost to clipping and the grid is never a power
+// of two coarser than it has to be.  x * 2^-e is exact, and a code is the
+// nearest magnitude, ties to the even code.
+//
+// Bound: HBM.  A value costs 4 bytes of f32 and 17/32 of a byte in the cache.
+// One lane takes eight values (32 bytes in, one dword of codes out), so a
+// block's largest magnitude is a maximum over four lanes (two DPP moves).  K's
+// dwords are contiguous over a wave; V's lie 16 bytes apart, the four tokens of
+// a group side by side, so a workgroup takes neighbouring tokens and the L2
+// merges their stores.
+#include <algorithm>
+
+#include "q4.hpp"
+
+namespace kore {
+
+constexpr int kQ4Block = 256;
+
+struct Q4Args {
+    const float* in[2];  // k, v (write)
+    float* out[2];       // k, v (read)
+    const uint32_t* slots;
+    uint8_t* cache;
+    uint64_t stride[2];  // floats between two tokens of k, v
+    uint64_t items;      // tokens * kv_heads * 4 nb
+    uint32_t head_dim;
+    Q4Cache c;
+};
+
+// Integer maximum over the four lanes of a block (quad_perm 1,0,3,2 and 2,3,0,1).
+__device__ __forceinline__ uint32_t quad_max(uint32_t v) {
+    v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0xb1, 0xf, 0xf, true));
+    return max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x4e, 0xf, 0xf, true));
+}
+
+// Item i -> token, key head, chunk of eight dimensions.
+__device__ __forceinline__ void q4_item(const Q4Args& a, uint64_t i, uint64_t* token, uint32_t* head, uint32_t* chunk) {
+    const uint32_t chunks = 4u * a.c.nb, row = chunks * a.c.kv_heads;
+    *token = i / row;
+    const uint32_t in_row = (uint32_t)(i - *token * row);
+    *head = in_row / chunks;
+    *chunk = in_row - *head * chunks;
+}
+
+__global__ __launch_bounds__(kQ4Block) void q4_write_kernel(Q4Args a) {
+    const uint64_t i = (uint64_t)blockIdx.x * kQ4Block + threadIdx.x;
+    const int which = blockIdx.y;  // 0: K, 1: V
+    if (i >= a.items) return;      // whole blocks of four lanes leave
+    uint64_t token;
+    uint32_t head, chunk;
+    q4_item(a, i, &token, &head, &chunk);
+    const float* row = a.in[which] + token * a.stride[which] + (uint64_t)head * a.head_dim;
+    const uint32_t d0 = chunk * 8u;
+    float x[8];
+    if (d0 + 8u <= a.head_dim) {
+        const f32x4 lo = *reinterpret_cast<const f32x4_a4*>(row + d0);
+        const f32x4 hi = *reinterpret_cast<const f32x4_a4*>(row + d0 + 4);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            x[j] = lo[j];
+            x[4 + j] = hi[j];
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = d0 + j < a.head_dim ? row[d0 + j] : 0.0f;
+    }
+    // The bits of |x| are ordered as their values, infinities and NaN last.
+    uint32_t amax = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) amax = max(amax, __float_as_uint(x[j]) & 0x7fffffffu);
+    amax = quad_max(amax);
+    const bool finite = amax < 0x7f800000u;
+    // Adding the mantissa of 2 - 1.75 carries exactly where amax > 1.75 * 2^x.
+    const int e = min(max((int)((amax + 0x1fffffu) >> 23) - 129, kQ4MinExp), kQ4MaxExp);
+    const float up = __uint_as_float((uint32_t)(127 - e) << 23);
+    // 3 * 2^126 is the largest magnitude that the top scale holds without overflow.
+    const float top = __uint_as_float(0x7f400000u);
+    uint32_t code = 0;
+    float y[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+        y[j] = fminf(fmaxf(fminf(fmaxf(x[j], -top), top) * up, -6.0f), 6.0f);
+    code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, y[0], y[1], 1.0f, 0);
+    code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, y[2], y[3], 1.0f, 1);
+    code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, y[4], y[5], 1.0f, 2);
+    code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, y[6], y[7], 1.0f, 3);
+    if (!finite) code = 0;
+    const uint32_t slot = a.slots[token];
+    const uint32_t page = slot >> a.c.shift, t = slot & (a.c.page - 1u);
+    if (page >= a.c.num_pages) return;
+    uint8_t* base = a.cache + (uint64_t)page * a.c.page_bytes + (uint64_t)head * a.c.head_bytes;
+    *reinterpret_cast<uint32_t*>(base + (which ? q4_v_code(a.c, t, chunk) : q4_k_code(a.c, t, chunk))) = code;
+    if ((chunk & 3u) == 0)
+        base[which ? q4_v_scale(a.c, t, chunk >> 2) : q4_k_scale(a.c, t, chunk >> 2)] =
+            (uint8_t)(finite ? (uint32_t)(e + 127) : kQ4NanScale);
+}
+
+__global__ __launch_bounds__(kQ4Block) void q4_read_kernel(Q4Args a) {
+    const uint64_t i = (uint64_t)blockIdx.x * kQ4Block + threadIdx.x;
+    const int which = blockIdx.y;
+    if (i >= a.items) return;
+    uint64_t token;
+    uint32_t head, chunk;
+    q4_item(a, i, &token, &head, &chunk);
+    const uint32_t slot = a.slots[token];
+    const uint32_t page = slot >> a.c.shift, t = slot & (a.c.page - 1u);
+    const uint32_t d0 = chunk * 8u;
+    if (d0 >= a.head_dim) return;
+    uint32_t code = 0, b = 127;
+    if (page < a.c.num_pages) {
+        const uint8_t* base = a.cache + (uint64_t)page * a.c.page_bytes + (uint64_t)head * a.c.head_bytes;
+        code = *reinterpret_cast<const uint32_t*>(base + (which ? q4_v_code(a.c, t, chunk) : q4_k_code(a.c, t, chunk)));
+        b = base[which ? q4_v_scale(a.c, t, chunk >> 2) : q4_k_scale(a.c, t, chunk >> 2)];
+    }
+    const float s = b == kQ4NanScale ? __uint_as_float(0x7fc00000u) : q4_scale(b);
+    f32x4 v[2];
+    auto p = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(code, 1.0f, 0);
+    v[0].x = p[0] * s;
+    v[0].y = p[1] * s;
+    p = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(code, 1.0f, 1);
+    v[0].z = p[0] * s;
+    v[0].w = p[1] * s;
+    p = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(code, 1.0f, 2);
+    v[1].x = p[0] * s;
+    v[1].y = p[1] * s;
+    p = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(code, 1.0f, 3);
+    v[1].z = p[0] * s;
+    v[1].w = p[1] * s;
+    float* row = a.out[which] + (token * a.c.kv_heads + head) * a.head_dim;
+    if (d0 + 8u <= a.head_dim) {
+        __builtin_nontemporal_store((f32x4_a4)v[0], reinterpret_cast<f32x4_a4*>(row + d0));
+        __builtin_nontemporal_store((f32x4_a4)v[1], reinterpret_cast<f32x4_a4*>(row + d0 + 4));
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (d0 + j < a.head_dim) row[d0 + j] = v[j >> 2][j & 3];
+    }
+}
+
+static bool overlap(const void* a, uint64_t na, const void* b, uint64_t nb) {
+    const char *p = (const char*)a, *q = (const char*)b;
+    return p < q + nb && q < p + na;
+}
+
+// Tokens in bands: a launch holds fewer than 2^32 threads.
+template <typename Kernel>
+static int q4_launch(Kernel kernel, Q4Args a, uint64_t tokens, bool write, hipStream_t s) {
+    const uint64_t per_token = (uint64_t)a.c.kv_heads * 4u * a.c.nb;
+    const uint64_t band = std::max<uint64_t>(1, (1ull << 30) / per_token);
+    for (uint64_t t = 0; t < tokens; t += band) {
+        const uint64_t n = std::min(band, tokens - t);
+        a.items = n * per_token;
+        hipLaunchKernelGGL(kernel, dim3((uint32_t)((a.items + kQ4Block - 1) / kQ4Block), 2), dim3(kQ4Block), 0, s, a);
+        const int st = launch_status();
+        if (st != KORE_HIP_OK) return st;
+        a.slots += n;
+        for (int w = 0; w < 2; ++w) {
+            if (write) a.in[w] += n * a.stride[w];
+            else a.out[w] += n * (uint64_t)a.c.kv_heads * a.head_dim;
+        }
+    }
+    return KORE_HIP_OK;
+}
+
+}  // namespace kore
+
+using namespace kore;
+
+extern "C" uint64_t kore_hip_kv_cache_q4_bytes(uint64_t num_pages, uint64_t page_size, uint64_t kv_heads,
+                                               uint64_t head_dim) {
+    Q4Cache c;
+    uint64_t bytes;
+    return q4_layout(num_pages, page_size, kv_heads, head_dim, &c, &bytes) == KORE_HIP_OK ? bytes : 0;
+}
+
+extern "C" int kore_hip_kv_cache_write_q4_f32(const float* k, const float* v, const uint32_t* slots, uint8_t* cache,
+                                              uint64_t tokens, uint64_t kv_heads, uint64_t head_dim,
+                                              uint64_t num_pages, uint64_t page_size, uint64_t k_stride,
+                                              uint64_t v_stride, kore_stream_t stream) {
+    if (tokens == 0 || kv_heads == 0 || head_dim == 0 || num_pages == 0) return KORE_HIP_OK;
+    Q4Args a = {};
+    uint64_t bytes, span[2];
+    const int st = q4_layout(num_pages, page_size, kv_heads, head_dim, &a.c, &bytes);
+    if (st != KORE_HIP_OK) return st;
+    if (!k || !v || !slots || !cache) return KORE_HIP_ERR_NULL_PTR;
+    if (!aligned16(cache)) return KORE_HIP_ERR_BAD_DIM;
+    const uint64_t row = kv_heads * head_dim;
+    a.stride[0] = k_stride ? k_stride : row;
+    a.stride[1] = v_stride ? v_stride : row;
+    for (int w = 0; w < 2; ++w) {
+        if (a.stride[w] < row) return KORE_HIP_ERR_BAD_DIM;
+        if (!mul_ok(tokens, a.stride[w], &span[w]) || span[w] > kMaxElements) return KORE_HIP_ERR_OVERFLOW;
+        span[w] = ((tokens - 1) * a.stride[w] + row) * 4;
+    }
+    if (overlap(cache, bytes, k, span[0]) || overlap(cache, bytes, v, span[1]) ||
+        overlap(cache, bytes, slots, tokens * 4))
+        return KORE_HIP_ERR_ALIAS;
+    a.in[0] = k;
+    a.in[1] = v;
+    a.slots = slots;
+    a.cache = cache;
+    a.head_dim = (uint32_t)head_dim;
+    return q4_launch(q4_write_kernel, a, tokens, true, (hipStream_t)stream);
+}
+
+extern "C" int kore_hip_kv_cache_read_q4_f32(const uint8_t* cache, const uint32_t* slots, float* k_out, float* v_out,
+                                             uint64_t tokens, uint64_t kv_heads, uint64_t head_dim,
+                                             uint64_t num_pages, uint64_t page_size, kore_stream_t stream) {
+    if (tokens == 0 || kv_heads == 0 || head_dim == 0) return KORE_HIP_OK;
+    Q4Args a = {};
+    uint64_t bytes, elems;
+    const int st = q4_layout(num_pages, page_size, kv_heads, head_dim, &a.c, &bytes);
+    if (st != KORE_HIP_OK) return st;
+    if (!slots || !k_out || !v_out || (num_pages && !cache)) return KORE_HIP_ERR_NULL_PTR;
+    if (num_pages && !aligned16(cache)) return KORE_HIP_ERR_BAD_DIM;
+    if (!mul_ok(tokens, kv_heads * head_dim, &elems) || elems > kMaxElements) return KORE_HIP_ERR_OVERFLOW;
+    if (overlap(k_out, elems * 4, v_out, elems * 4) || overlap(cache, bytes, k_out, elems * 4) ||
+        overlap(cache, bytes, v_out, elems * 4) || overlap(slots, tokens * 4, k_out, elems * 4) ||
+        overlap(slots, tokens * 4, v_out, elems * 4))
+        return KORE_HIP_ERR_ALIAS;
+    a.out[0] = k_out;
+    a.out[1] = v_out;
+    a.slots = slots;
+    a.cache = const_cast<uint8_t*>(cache);
+    a.head_dim = (uint32_t)head_dim;
+    return q4_launch(q4_read_kernel, a, tokens, false, (hipStream_t)stream);
+}

@@ -506,3 +506,167 @@ def rocm_pack_weights_ternary(device_idx: int, w: HipBuffer, m: int, k: int, thr
 
 __all__ += ["rocm_ternary_matmul_i8", "rocm_ternary_matmul_f32", "rocm_bit_linear_f32", "rocm_bit_linear_i8",
             "rocm_pack_weights_ternary"]
+
+
+# ------------------------------------------- query/key norm with rotation
+def _rows(tokens: int, stride: int, row: int) -> int:
+    """Bytes from a token's first float to the last token's end (stride 0: contiguous rows)."""
+    return ((tokens - 1) * (stride or row) + row) * 4 if tokens and row else 0
+
+
+def rocm_qk_norm_rope_f32(device_idx: int, q: HipBuffer, k: HipBuffer, q_weight: HipBuffer, k_weight: HipBuffer,
+                          inv_freq: HipBuffer, batch: int, seq_len: int, q_heads: int, k_heads: int, head_dim: int,
+                          eps: float, start_pos: int = 0, positions: Optional[HipBuffer] = None,
+                          interleaved: bool = False, q_stride: int = 0, k_stride: int = 0,
+                          q_out: Optional[HipBuffer] = None, k_out: Optional[HipBuffer] = None,
+                          q_out_stride: int = 0, k_out_stride: int = 0) -> Tuple[HipBuffer, HipBuffer]:
+    """RMSNorm of every Q and K head and the rotation in one pass (the
+    reference composes cpu_fused.rs:160-190 with kore-edge's
+    ``apply_rope``).  Tokens lie ``*_stride`` floats apart (0: contiguous), so
+    q and k may be parts of a fused projection's output; ``positions`` (u32 per
+    token) replaces ``start_pos + s``.  Returns (q_out, k_out); q and k
+    themselves may be given for in-place work."""
+    lib = _library(device_idx)
+    t = batch * seq_len
+    _need(q, _rows(t, q_stride, q_heads * head_dim), "qk_norm_rope q")
+    _need(k, _rows(t, k_stride, k_heads * head_dim), "qk_norm_rope k")
+    _need(q_weight, head_dim * 4 if q_heads else 0, "qk_norm_rope q_weight")
+    _need(k_weight, head_dim * 4 if k_heads else 0, "qk_norm_rope k_weight")
+    _need(inv_freq, (head_dim // 2) * 4, "qk_norm_rope inv_freq")
+    if positions is not None:
+        _need(positions, t * 4, "qk_norm_rope positions")
+    qo = _out(device_idx, q_out, _rows(t, q_out_stride, q_heads * head_dim), "qk_norm_rope q_out")
+    ko = _out(device_idx, k_out, _rows(t, k_out_stride, k_heads * head_dim), "qk_norm_rope k_out")
+    _check(lib.kore_hip_qk_norm_rope_f32(q.ptr, k.ptr, q_weight.ptr, k_weight.ptr, inv_freq.ptr,
+                                         positions.ptr if positions is not None else None, qo.ptr, ko.ptr, batch,
+                                         seq_len, q_heads, k_heads, head_dim, q_stride, k_stride, q_out_stride,
+                                         k_out_stride, start_pos, eps, int(bool(interleaved)), _stream(device_idx)),
+           "qk_norm_rope_f32")
+    return qo, ko
+
+
+def rocm_qk_norm_rope_backward_workspace_bytes(tokens: int, q_heads: int, k_heads: int, head_dim: int) -> int:
+    """Device scratch ``rocm_qk_norm_rope_backward_f32`` needs."""
+    return int(_lib.load().kore_hip_qk_norm_rope_backward_workspace_bytes(tokens, q_heads, k_heads, head_dim))
+
+
+def rocm_qk_norm_rope_backward_f32(device_idx: int, grad_q_out: HipBuffer, grad_k_out: HipBuffer, q: HipBuffer,
+                                   k: HipBuffer, q_weight: HipBuffer, k_weight: HipBuffer, inv_freq: HipBuffer,
+                                   batch: int, seq_len: int, q_heads: int, k_heads: int, head_dim: int, eps: float,
+                                   start_pos: int = 0, positions: Optional[HipBuffer] = None,
+                                   interleaved: bool = False, q_stride: int = 0, k_stride: int = 0,
+                                   workspace: Optional[HipBuffer] = None, grad_q: Optional[HipBuffer] = None,
+                                   grad_k: Optional[HipBuffer] = None, grad_q_weight: Optional[HipBuffer] = None,
+                                   grad_k_weight: Optional[HipBuffer] = None, grad_q_out_stride: int = 0,
+                                   grad_k_out_stride: int = 0, grad_q_stride: int = 0, grad_k_stride: int = 0):
+    """Backward of ``rocm_qk_norm_rope_f32`` -> (grad_q, grad_k,
+    grad_q_weight, grad_k_weight).  The workspace is allocated when not given."""
+    lib = _library(device_idx)
+    t = batch * seq_len
+    rq, rk = q_heads * head_dim, k_heads * head_dim
+    _need(grad_q_out, _rows(t, grad_q_out_stride, rq), "qk_norm_rope_backward grad_q_out")
+    _need(grad_k_out, _rows(t, grad_k_out_stride, rk), "qk_norm_rope_backward grad_k_out")
+    _need(q, _rows(t, q_stride, rq), "qk_norm_rope_backward q")
+    _need(k, _rows(t, k_stride, rk), "qk_norm_rope_backward k")
+    _need(q_weight, head_dim * 4 if q_heads else 0, "qk_norm_rope_backward q_weight")
+    _need(k_weight, head_dim * 4 if k_heads else 0, "qk_norm_rope_backward k_weight")
+    _need(inv_freq, (head_dim // 2) * 4, "qk_norm_rope_backward inv_freq")
+    if positions is not None:
+        _need(positions, t * 4, "qk_norm_rope_backward positions")
+    gq = _out(device_idx, grad_q, _rows(t, grad_q_stride, rq), "qk_norm_rope_backward grad_q")
+    gk = _out(device_idx, grad_k, _rows(t, grad_k_stride, rk), "qk_norm_rope_backward grad_k")
+    gqw = _out(device_idx, grad_q_weight, head_dim * 4 if q_heads else 0, "qk_norm_rope_backward grad_q_weight")
+    gkw = _out(device_idx, grad_k_weight, head_dim * 4 if k_heads else 0, "qk_norm_rope_backward grad_k_weight")
+    ws = workspace if workspace is not None else HipBuffer.empty(device_idx, max(
+        16, rocm_qk_norm_rope_backward_workspace_bytes(t, q_heads, k_heads, head_dim)))
+    _check(lib.kore_hip_qk_norm_rope_backward_f32(
+        grad_q_out.ptr, grad_k_out.ptr, q.ptr, k.ptr, q_weight.ptr, k_weight.ptr, inv_freq.ptr,
+        positions.ptr if positions is not None else None, gq.ptr, gk.ptr, gqw.ptr, gkw.ptr, ws.ptr, ws.nbytes, batch,
+        seq_len, q_heads, k_heads, head_dim, grad_q_out_stride, grad_k_out_stride, q_stride, k_stride, grad_q_stride,
+        grad_k_stride, start_pos, eps, int(bool(interleaved)), _stream(device_idx)), "qk_norm_rope_backward_f32")
+    return gq, gk, gqw, gkw
+
+
+# --------------------------------------------------- 4-bit key/value cache
+def rocm_kv_cache_q4_bytes(num_pages: int, page_size: int, kv_heads: int, head_dim: int) -> int:
+    """Size of one layer's 4-bit cache (include/kore_hip.h has its layout)."""
+    n = int(_lib.load().kore_hip_kv_cache_q4_bytes(num_pages, page_size, kv_heads, head_dim))
+    if not n and num_pages and kv_heads:
+        raise RocmError("LaunchError", f"kv_cache_q4: no cache of {num_pages} pages of {page_size} tokens, "
+                        f"{kv_heads} heads of {head_dim}")
+    return n
+
+
+def rocm_kv_cache_write_q4_f32(device_idx: int, k: HipBuffer, v: HipBuffer, slots: HipBuffer, cache: HipBuffer,
+                               tokens: int, kv_heads: int, head_dim: int, num_pages: int, page_size: int,
+                               k_stride: int = 0, v_stride: int = 0) -> None:
+    """Quantises K and V of ``tokens`` tokens into their slots (u32, page *
+    page_size + token of the page; one past the last page is skipped).  The
+    device twin of a KV cache's append (crates/kore-attention/src/kv_cache.rs:11,
+    f32 there)."""
+    lib = _library(device_idx)
+    row = kv_heads * head_dim
+    _need(k, _rows(tokens, k_stride, row), "kv_cache_write k")
+    _need(v, _rows(tokens, v_stride, row), "kv_cache_write v")
+    _need(slots, tokens * 4, "kv_cache_write slots")
+    _need(cache, lib.kore_hip_kv_cache_q4_bytes(num_pages, page_size, kv_heads, head_dim), "kv_cache_write cache")
+    _check(lib.kore_hip_kv_cache_write_q4_f32(k.ptr, v.ptr, slots.ptr, cache.ptr, tokens, kv_heads, head_dim,
+                                              num_pages, page_size, k_stride, v_stride, _stream(device_idx)),
+           "kv_cache_write_q4_f32")
+
+
+def rocm_kv_cache_read_q4_f32(device_idx: int, cache: HipBuffer, slots: HipBuffer, tokens: int, kv_heads: int,
+                              head_dim: int, num_pages: int, page_size: int, k_out: Optional[HipBuffer] = None,
+                              v_out: Optional[HipBuffer] = None) -> Tuple[HipBuffer, HipBuffer]:
+    """The cached values of ``tokens`` slots as f32 (k, v) [tokens, kv_heads, head_dim]."""
+    lib = _library(device_idx)
+    n = tokens * kv_heads * head_dim * 4
+    _need(slots, tokens * 4, "kv_cache_read slots")
+    _need(cache, lib.kore_hip_kv_cache_q4_bytes(num_pages, page_size, kv_heads, head_dim), "kv_cache_read cache")
+    ko = _out(device_idx, k_out, n, "kv_cache_read k_out")
+    vo = _out(device_idx, v_out, n, "kv_cache_read v_out")
+    _check(lib.kore_hip_kv_cache_read_q4_f32(cache.ptr, slots.ptr, ko.ptr, vo.ptr, tokens, kv_heads, head_dim,
+                                             num_pages, page_size, _stream(device_idx)), "kv_cache_read_q4_f32")
+    return ko, vo
+
+
+def rocm_attention_q4_workspace_bytes(num_seqs: int, tokens: int, q_heads: int, kv_heads: int, head_dim: int,
+                                      page_size: int, max_pages: int) -> int:
+    """Device scratch ``rocm_attention_q4_f32`` needs (0 for some sizes)."""
+    return int(_lib.load().kore_hip_attention_q4_workspace_bytes(num_seqs, tokens, q_heads, kv_heads, head_dim,
+                                                                 page_size, max_pages))
+
+
+def rocm_attention_q4_f32(device_idx: int, q: HipBuffer, cache: HipBuffer, page_table: HipBuffer, kv_lens: HipBuffer,
+                          q_starts: HipBuffer, num_seqs: int, tokens: int, q_heads: int, kv_heads: int, head_dim: int,
+                          num_pages: int, page_size: int, max_pages: int, scale: float, causal: bool = True,
+                          q_stride: int = 0, workspace: Optional[HipBuffer] = None,
+                          out: Optional[HipBuffer] = None) -> HipBuffer:
+    """softmax(scale q k^T) v over each sequence's pages of the 4-bit cache:
+    ``num_seqs`` ragged sequences, sequence s with query tokens
+    q_starts[s]..q_starts[s+1] and kv_lens[s] cached tokens (its new ones
+    written already), query heads sharing key heads.  The reference attends in
+    f32 on the CPU (crates/kore-attention/src/flash.rs:28).  Returns
+    out[tokens, q_heads, head_dim]; rows of no sequence are left as they are.
+    The workspace is allocated when not given."""
+    lib = _library(device_idx)
+    row = q_heads * head_dim
+    _need(q, _rows(tokens, q_stride, row), "attention q")
+    _need(cache, lib.kore_hip_kv_cache_q4_bytes(num_pages, page_size, kv_heads, head_dim), "attention cache")
+    _need(page_table, num_seqs * max_pages * 4, "attention page_table")
+    _need(kv_lens, num_seqs * 4, "attention kv_lens")
+    _need(q_starts, (num_seqs + 1) * 4 if num_seqs else 0, "attention q_starts")
+    o = _out(device_idx, out, tokens * row * 4, "attention out")
+    if workspace is None:
+        workspace = HipBuffer.empty(device_idx, max(16, lib.kore_hip_attention_q4_workspace_bytes(
+            num_seqs, tokens, q_heads, kv_heads, head_dim, page_size, max_pages)))
+    _check(lib.kore_hip_attention_q4_f32(q.ptr, cache.ptr, page_table.ptr, kv_lens.ptr, q_starts.ptr, o.ptr,
+                                         workspace.ptr, workspace.nbytes, num_seqs, tokens, q_heads, kv_heads,
+                                         head_dim, num_pages, page_size, max_pages, q_stride, scale,
+                                         int(bool(causal)), _stream(device_idx)), "attention_q4_f32")
+    return o
+
+
+__all__ += ["rocm_qk_norm_rope_f32", "rocm_qk_norm_rope_backward_workspace_bytes", "rocm_qk_norm_rope_backward_f32",
+            "rocm_kv_cache_q4_bytes", "rocm_kv_cache_write_q4_f32", "rocm_kv_cache_read_q4_f32",
+            "rocm_attention_q4_workspace_bytes", "rocm_attention_q4_f32"]

@@ -50,6 +50,23 @@ type FnBitLinearF32 = unsafe extern "C" fn(*const u8, *const f32, *const f32, *c
 type FnBitLinearI8 = unsafe extern "C" fn(*const u8, *const f32, *const i8, *const f32, *const f32, *mut f32, u64,
                                          u64, u64, Stream) -> c_int;
 type FnPackTernary = unsafe extern "C" fn(*const f32, u64, u64, f32, *mut u8, *mut f32, Stream) -> c_int;
+type FnQkNormRope = unsafe extern "C" fn(*const f32, *const f32, *const f32, *const f32, *const f32, *const u32,
+                                         *mut f32, *mut f32, u64, u64, u32, u32, u32, u64, u64, u64, u64, u64, f32,
+                                         c_int, Stream) -> c_int;
+type FnQkNormRopeBwdWs = unsafe extern "C" fn(u64, u32, u32, u32) -> u64;
+type FnQkNormRopeBwd = unsafe extern "C" fn(*const f32, *const f32, *const f32, *const f32, *const f32, *const f32,
+                                            *const f32, *const u32, *mut f32, *mut f32, *mut f32, *mut f32, *mut f32,
+                                            u64, u64, u64, u32, u32, u32, u64, u64, u64, u64, u64, u64, u64, f32,
+                                            c_int, Stream) -> c_int;
+type FnCacheBytes = unsafe extern "C" fn(u64, u64, u64, u64) -> u64;
+type FnCacheWrite = unsafe extern "C" fn(*const f32, *const f32, *const u32, *mut u8, u64, u64, u64, u64, u64, u64,
+                                         u64, Stream) -> c_int;
+type FnCacheRead = unsafe extern "C" fn(*const u8, *const u32, *mut f32, *mut f32, u64, u64, u64, u64, u64,
+                                        Stream) -> c_int;
+type FnAttentionWs = unsafe extern "C" fn(u64, u64, u64, u64, u64, u64, u64) -> u64;
+type FnAttention = unsafe extern "C" fn(*const f32, *const u8, *const u32, *const u32, *const u32, *mut f32, *mut f32,
+                                        u64, u64, u64, u64, u64, u64, u64, u64, u64, u64, f32, c_int,
+                                        Stream) -> c_int;
 type FnStatus = unsafe extern "C" fn(c_int) -> *const c_char;
 
 struct FusedApi {
@@ -79,6 +96,14 @@ struct FusedApi {
     bit_linear_f32: FnBitLinearF32,
     bit_linear_i8: FnBitLinearI8,
     pack_ternary: FnPackTernary,
+    qk_norm_rope: FnQkNormRope,
+    qk_norm_rope_bwd_ws: FnQkNormRopeBwdWs,
+    qk_norm_rope_bwd: FnQkNormRopeBwd,
+    kv_cache_bytes: FnCacheBytes,
+    kv_cache_write: FnCacheWrite,
+    kv_cache_read: FnCacheRead,
+    attention_ws: FnAttentionWs,
+    attention: FnAttention,
     status: FnStatus,
 }
 unsafe impl Send for FusedApi {}
@@ -116,6 +141,14 @@ fn api() -> Result<&'static FusedApi, RocmError> {
             bit_linear_f32: *lib.get(b"kore_hip_bit_linear_f32\0").ok()?,
             bit_linear_i8: *lib.get(b"kore_hip_bit_linear_i8\0").ok()?,
             pack_ternary: *lib.get(b"kore_hip_pack_weights_ternary\0").ok()?,
+            qk_norm_rope: *lib.get(b"kore_hip_qk_norm_rope_f32\0").ok()?,
+            qk_norm_rope_bwd_ws: *lib.get(b"kore_hip_qk_norm_rope_backward_workspace_bytes\0").ok()?,
+            qk_norm_rope_bwd: *lib.get(b"kore_hip_qk_norm_rope_backward_f32\0").ok()?,
+            kv_cache_bytes: *lib.get(b"kore_hip_kv_cache_q4_bytes\0").ok()?,
+            kv_cache_write: *lib.get(b"kore_hip_kv_cache_write_q4_f32\0").ok()?,
+            kv_cache_read: *lib.get(b"kore_hip_kv_cache_read_q4_f32\0").ok()?,
+            attention_ws: *lib.get(b"kore_hip_attention_q4_workspace_bytes\0").ok()?,
+            attention: *lib.get(b"kore_hip_attention_q4_f32\0").ok()?,
             status: *lib.get(b"kore_hip_status_string\0").ok()?,
             _lib: lib,
         })
@@ -479,4 +512,184 @@ pub fn rocm_pack_weights_ternary(dev: usize, w: &HipBuffer, m: usize, k: usize, 
                                          packed.as_device_ptr() as _, scales.as_device_ptr() as _,
                                          std::ptr::null_mut()) }, "pack_weights_ternary")?;
     Ok((packed, scales))
+}
+
+/// Shape of `rocm_qk_norm_rope_f32` and its backward.  Tokens of q and k lie `q_stride` / `k_stride`
+/// floats apart (0: contiguous); the other tensors are contiguous.
+#[derive(Clone, Copy)]
+pub struct QkShape {
+    pub batch: usize,
+    pub seq_len: usize,
+    pub q_heads: usize,
+    pub k_heads: usize,
+    pub head_dim: usize,
+    pub q_stride: usize,
+    pub k_stride: usize,
+    pub start_pos: usize,
+    pub interleaved: bool,
+}
+
+impl QkShape {
+    fn tokens(&self) -> Result<usize, RocmError> {
+        prod(&[self.batch, self.seq_len])
+    }
+
+    /// Bytes of one contiguous tensor of `heads` heads.
+    fn bytes(&self, heads: usize) -> Result<usize, RocmError> {
+        prod(&[self.batch, self.seq_len, heads, self.head_dim, 4])
+    }
+
+    fn check(&self, q: &HipBuffer, k: &HipBuffer, qw: &HipBuffer, kw: &HipBuffer, inv_freq: &HipBuffer,
+             positions: Option<&HipBuffer>) -> Result<(), RocmError> {
+        let t = self.tokens()?;
+        need(q, span(t, self.q_stride, prod(&[self.q_heads, self.head_dim])?)?, "qk_norm_rope q")?;
+        need(k, span(t, self.k_stride, prod(&[self.k_heads, self.head_dim])?)?, "qk_norm_rope k")?;
+        need(qw, prod(&[self.head_dim, 4])?, "qk_norm_rope q_weight")?;
+        need(kw, prod(&[self.head_dim, 4])?, "qk_norm_rope k_weight")?;
+        need(inv_freq, prod(&[self.head_dim / 2, 4])?, "qk_norm_rope inv_freq")?;
+        if let Some(p) = positions {
+            need(p, prod(&[t, 4])?, "qk_norm_rope positions")?;
+        }
+        Ok(())
+    }
+}
+
+/// Bytes from a token's first float to the last token's end.
+fn span(tokens: usize, stride: usize, row: usize) -> Result<usize, RocmError> {
+    if tokens == 0 || row == 0 {
+        return Ok(0);
+    }
+    let s = if stride == 0 { row } else { stride };
+    prod(&[prod(&[tokens - 1, s])?.checked_add(row).unwrap_or(usize::MAX), 4])
+}
+
+/// RMSNorm of every Q and K head and the rotation in one pass (cpu_fused.rs:160-190 per head, then
+/// kore-edge's `apply_rope`, which the reference runs apart): (q_out, k_out), contiguous.
+pub fn rocm_qk_norm_rope_f32(dev: usize, q: &HipBuffer, k: &HipBuffer, q_weight: &HipBuffer, k_weight: &HipBuffer,
+                             inv_freq: &HipBuffer, positions: Option<&HipBuffer>, s: QkShape, eps: f32)
+                             -> Result<(HipBuffer, HipBuffer), RocmError> {
+    s.check(q, k, q_weight, k_weight, inv_freq, positions)?;
+    set_device(dev)?;
+    let qo = HipBuffer::zeros(dev, s.bytes(s.q_heads)?)?;
+    let ko = HipBuffer::zeros(dev, s.bytes(s.k_heads)?)?;
+    let pp = positions.map_or(std::ptr::null(), |p| p.as_device_ptr() as *const u32);
+    check(unsafe { (api()?.qk_norm_rope)(q.as_device_ptr() as _, k.as_device_ptr() as _,
+                                         q_weight.as_device_ptr() as _, k_weight.as_device_ptr() as _,
+                                         inv_freq.as_device_ptr() as _, pp, qo.as_device_ptr() as _,
+                                         ko.as_device_ptr() as _, s.batch as u64, s.seq_len as u64,
+                                         s.q_heads as u32, s.k_heads as u32, s.head_dim as u32, s.q_stride as u64,
+                                         s.k_stride as u64, 0, 0, s.start_pos as u64, eps, s.interleaved as c_int,
+                                         std::ptr::null_mut()) }, "qk_norm_rope_f32")?;
+    Ok((qo, ko))
+}
+
+/// Its backward: (grad_q, grad_k, grad_q_weight, grad_k_weight), contiguous.  This wrapper allocates
+/// the workspace.
+pub fn rocm_qk_norm_rope_backward_f32(dev: usize, grad_q_out: &HipBuffer, grad_k_out: &HipBuffer, q: &HipBuffer,
+                                      k: &HipBuffer, q_weight: &HipBuffer, k_weight: &HipBuffer,
+                                      inv_freq: &HipBuffer, positions: Option<&HipBuffer>, s: QkShape, eps: f32)
+                                      -> Result<(HipBuffer, HipBuffer, HipBuffer, HipBuffer), RocmError> {
+    s.check(q, k, q_weight, k_weight, inv_freq, positions)?;
+    need(grad_q_out, s.bytes(s.q_heads)?, "qk_norm_rope_backward grad_q_out")?;
+    need(grad_k_out, s.bytes(s.k_heads)?, "qk_norm_rope_backward grad_k_out")?;
+    set_device(dev)?;
+    let gq = HipBuffer::zeros(dev, s.bytes(s.q_heads)?)?;
+    let gk = HipBuffer::zeros(dev, s.bytes(s.k_heads)?)?;
+    let gqw = HipBuffer::zeros(dev, prod(&[s.head_dim, 4])?)?;
+    let gkw = HipBuffer::zeros(dev, prod(&[s.head_dim, 4])?)?;
+    let wsb = unsafe { (api()?.qk_norm_rope_bwd_ws)(s.tokens()? as u64, s.q_heads as u32, s.k_heads as u32,
+                                                    s.head_dim as u32) } as usize;
+    let ws = HipBuffer::zeros(dev, wsb.max(16))?;
+    let pp = positions.map_or(std::ptr::null(), |p| p.as_device_ptr() as *const u32);
+    check(unsafe { (api()?.qk_norm_rope_bwd)(grad_q_out.as_device_ptr() as _, grad_k_out.as_device_ptr() as _,
+                                             q.as_device_ptr() as _, k.as_device_ptr() as _,
+                                             q_weight.as_device_ptr() as _, k_weight.as_device_ptr() as _,
+                                             inv_freq.as_device_ptr() as _, pp, gq.as_device_ptr() as _,
+                                             gk.as_device_ptr() as _, gqw.as_device_ptr() as _,
+                                             gkw.as_device_ptr() as _, ws.as_device_ptr() as _, ws.len() as u64,
+                                             s.batch as u64, s.seq_len as u64, s.q_heads as u32, s.k_heads as u32,
+                                             s.head_dim as u32, 0, 0, s.q_stride as u64, s.k_stride as u64, 0, 0,
+                                             s.start_pos as u64, eps, s.interleaved as c_int,
+                                             std::ptr::null_mut()) }, "qk_norm_rope_backward_f32")?;
+    Ok((gq, gk, gqw, gkw))
+}
+
+/// One layer's 4-bit key/value cache: `num_pages` pages of `page_size` tokens.
+pub struct KvCacheQ4 {
+    pub buf: HipBuffer,
+    pub num_pages: usize,
+    pub page_size: usize,
+    pub kv_heads: usize,
+    pub head_dim: usize,
+}
+
+impl KvCacheQ4 {
+    pub fn new(dev: usize, num_pages: usize, page_size: usize, kv_heads: usize, head_dim: usize)
+               -> Result<Self, RocmError> {
+        let n = unsafe { (api()?.kv_cache_bytes)(num_pages as u64, page_size as u64, kv_heads as u64,
+                                                 head_dim as u64) } as usize;
+        if n == 0 {
+            return Err(RocmError::MemoryError(format!(
+                "kv_cache_q4: no cache of {num_pages} pages of {page_size} tokens, {kv_heads} heads of {head_dim}")));
+        }
+        Ok(Self { buf: HipBuffer::zeros(dev, n)?, num_pages, page_size, kv_heads, head_dim })
+    }
+
+    /// Quantises K and V[tokens, kv_heads, head_dim] into slots (u32: page * page_size + token of
+    /// the page; one past the last page is skipped).
+    pub fn write(&self, dev: usize, k: &HipBuffer, v: &HipBuffer, slots: &HipBuffer, tokens: usize, k_stride: usize,
+                 v_stride: usize) -> Result<(), RocmError> {
+        let row = prod(&[self.kv_heads, self.head_dim])?;
+        need(k, span(tokens, k_stride, row)?, "kv_cache_write k")?;
+        need(v, span(tokens, v_stride, row)?, "kv_cache_write v")?;
+        need(slots, prod(&[tokens, 4])?, "kv_cache_write slots")?;
+        set_device(dev)?;
+        check(unsafe { (api()?.kv_cache_write)(k.as_device_ptr() as _, v.as_device_ptr() as _,
+                                               slots.as_device_ptr() as _, self.buf.as_device_ptr() as _,
+                                               tokens as u64, self.kv_heads as u64, self.head_dim as u64,
+                                               self.num_pages as u64, self.page_size as u64, k_stride as u64,
+                                               v_stride as u64, std::ptr::null_mut()) }, "kv_cache_write_q4_f32")
+    }
+
+    /// The cached values of `tokens` slots: (k, v)[tokens, kv_heads, head_dim].
+    pub fn read(&self, dev: usize, slots: &HipBuffer, tokens: usize) -> Result<(HipBuffer, HipBuffer), RocmError> {
+        need(slots, prod(&[tokens, 4])?, "kv_cache_read slots")?;
+        let n = prod(&[tokens, self.kv_heads, self.head_dim, 4])?;
+        set_device(dev)?;
+        let (k, v) = (HipBuffer::zeros(dev, n)?, HipBuffer::zeros(dev, n)?);
+        check(unsafe { (api()?.kv_cache_read)(self.buf.as_device_ptr() as _, slots.as_device_ptr() as _,
+                                              k.as_device_ptr() as _, v.as_device_ptr() as _, tokens as u64,
+                                              self.kv_heads as u64, self.head_dim as u64, self.num_pages as u64,
+                                              self.page_size as u64, std::ptr::null_mut()) },
+              "kv_cache_read_q4_f32")?;
+        Ok((k, v))
+    }
+
+    /// softmax(scale q k^T) v for `num_seqs` ragged sequences: page_table[num_seqs][max_pages],
+    /// kv_lens[num_seqs], q_starts[num_seqs + 1], all u32.  This wrapper allocates the workspace.
+    #[allow(clippy::too_many_arguments)]
+    pub fn attend(&self, dev: usize, q: &HipBuffer, page_table: &HipBuffer, kv_lens: &HipBuffer,
+                  q_starts: &HipBuffer, num_seqs: usize, tokens: usize, q_heads: usize, max_pages: usize,
+                  q_stride: usize, scale: f32, causal: bool) -> Result<HipBuffer, RocmError> {
+        let row = prod(&[q_heads, self.head_dim])?;
+        need(q, span(tokens, q_stride, row)?, "attention q")?;
+        need(page_table, prod(&[num_seqs, max_pages, 4])?, "attention page_table")?;
+        need(kv_lens, prod(&[num_seqs, 4])?, "attention kv_lens")?;
+        need(q_starts, prod(&[num_seqs.checked_add(1).unwrap_or(usize::MAX), 4])?, "attention q_starts")?;
+        set_device(dev)?;
+        let out = HipBuffer::zeros(dev, prod(&[tokens, row, 4])?)?;
+        let wsb = unsafe { (api()?.attention_ws)(num_seqs as u64, tokens as u64, q_heads as u64,
+                                                 self.kv_heads as u64, self.head_dim as u64, self.page_size as u64,
+                                                 max_pages as u64) } as usize;
+        let ws = HipBuffer::zeros(dev, wsb.max(16))?;
+        check(unsafe { (api()?.attention)(q.as_device_ptr() as _, self.buf.as_device_ptr() as _,
+                                          page_table.as_device_ptr() as _, kv_lens.as_device_ptr() as _,
+                                          q_starts.as_device_ptr() as _, out.as_device_ptr() as _,
+                                          ws.as_device_ptr() as _, ws.len() as u64, num_seqs as u64, tokens as u64,
+                                          q_heads as u64, self.kv_heads as u64, self.head_dim as u64,
+                                          self.num_pages as u64, self.page_size as u64, max_pages as u64,
+                                          q_stride as u64, scale, causal as c_int, std::ptr::null_mut()) },
+              "attention_q4_f32")?;
+        Ok(out)
+    }
 }
