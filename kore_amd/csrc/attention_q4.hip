@@ -5,17 +5,19 @@
 // scores in memory.  The rows of one key head are its query heads times the
 // sequence's new tokens: row r = token * group + head, 16 to a matrix tile.
 //
-// Arithmetic.  A cached value is a code times a power of two, exact in bf16, so
-// the matrix cores' bf16 form loses nothing on the cache's side.  A query value
-// (times scale * log2 e, one f32 rounding) is cut into three bf16 terms of 8
-// bits each, which is all of its 24: every product q * k is exact and sums are
-// f32.  A probability is two bf16 terms rounded to nearest: it is off by at
-// most 2^-18 of itself, half of what a term of 16 bits leaves, next to the few
-// f32 roundings in the score that it is the exponential of; the row's sum takes
-// the f32 value.
+// Arithmetic.  A cached value is a code times a power of two, exact in bf16, and
+// gfx950 makes two of them with their scale in one instruction, so the matrix
+// cores' bf16 form loses nothing on the cache's side.  A query value (times scale
+// * log2 e, one f32 rounding) is cut into three bf16 terms of 8 bits each, which
+// is all of its 24: every product q * k is exact and sums are f32.  A probability
+// is two bf16 terms rounded to nearest: it is off by at most 2^-18 of itself, next
+// to the few f32 roundings of the score that it is the exponential of; the row's
+// sum takes the f32 value.
+// (The block-scaled product takes K's codes and scales as they lie, and q as six
+// E4M3 terms; but its sum keeps only some 2^-19 of the largest product, so blocks
+// of very different scales would cost accuracy that f32 has.)
 //
-// Layout of a step (32 tokens, v_mfma_f32_16x16x32_bf16; n = lane % 16,
-// g = lane / 16):
+// Layout of a step (32 tokens; n = lane % 16, g = lane / 16):
 //   S^T = K Q^T   a lane holds token n's dimensions of group g (K's codes as
 //                 they lie, 16 bytes at head_dim 128) and row n's same
 //                 dimensions: which eight of them meet in one product is free.
@@ -32,6 +34,7 @@
 // that only later rows see is NaN, the product uses 1 for the scale and the
 // rows that see it are set to NaN one by one.
 #include <algorithm>
+#include <type_traits>
 
 #include "q4.hpp"
 
@@ -44,7 +47,11 @@ typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 constexpr int kAttBlock = 256;
 constexpr int kAttWaves = kAttBlock / kWave;
 constexpr uint32_t kAttStep = 32;      // tokens of a step
-constexpr uint32_t kAttCombine = 256;  // threads of the joining kernel
+constexpr uint32_t kAttMinChunk = 8;   // steps of a split, at least
+constexpr uint32_t kAttMaxSteps = 1u << 27;  // more than 2^31 keys have
+constexpr int kAttTerms = 3;           // bf16 terms of a query value
+constexpr uint32_t kAttJoin = 512;  // threads of the joining kernel
+constexpr uint32_t kAttMaxSplits = 1024;
 
 struct AttArgs {
     const float* q;
@@ -56,70 +63,121 @@ struct AttArgs {
     float* part;
     uint64_t q_stride;
     uint64_t tokens;
-    uint32_t num_seqs, q_heads, group, max_pages, dim, tiles, tile0, splits;
+    uint32_t num_seqs, q_heads, group, max_pages, dim;
+    uint32_t items, item0;  // work items there can be (see att_item), first of this launch
+    uint32_t target;        // items to cut the keys into, 0: one a tile
     float scale_log2;
     int causal;
     Q4Cache c;
 };
 
-// A tile: `rows` consecutive rows of one sequence and key head.
-struct AttTile {
-    uint32_t seq, q0, q_len, kv_len, first;  // first: its first row in the sequence
-    uint32_t rows;                           // rows of the sequence
+// A work item: kRows consecutive rows of one sequence and one share of its keys.
+struct AttItem {
+    uint32_t seq, q0, q_len, kv_len;
+    uint32_t rows, first;    // rows of the sequence, the tile's first
+    uint32_t chunk, split;   // steps of a share, the item's share
+    uint32_t splits;         // shares of the sequence's keys
     bool ok;
 };
 
-// Sequence s owns tiles from start_s * group / kRows + s on: its
-// ceil(len * group / kRows) tiles end before the next sequence's first, so a
-// tile's number alone names it.  Tiles between are empty.
+// Inclusive sum over the wave's lanes (row_shr 1, 2, 4, 8 and the rows' last
+// lanes broadcast on).
+__device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x111, 0xf, 0xf, false);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x112, 0xf, 0xf, false);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x114, 0xf, 0xf, false);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x118, 0xf, 0xf, false);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xa, 0xf, false);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xc, 0xf, false);
+    return v;
+}
+
+__device__ __forceinline__ uint32_t wave_total(uint32_t v) {
+    return (uint32_t)__builtin_amdgcn_readlane((int)wave_scan(v), kWave - 1);
+}
+
+__device__ __forceinline__ uint32_t att_steps(uint32_t keys) { return (keys + kAttStep - 1) / kAttStep; }
+
+// Items are numbered through the sequences: a sequence has ceil(len * group /
+// kRows) tiles of ceil(steps / chunk) shares each.  The chunk is the same for all
+// sequences, so that items take equally long however ragged the lengths are: the
+// least (to an eighth) with which there are no more than `target`.  The host
+// knows no lengths; the grid has as many items as there can be, and those past
+// the last are empty.
 template <uint32_t kRows>
-__device__ __forceinline__ AttTile att_tile(const AttArgs& a, uint32_t tile) {
-    AttTile t = {};
-    uint32_t before = 0;
-    for (uint32_t s0 = 0; s0 < a.num_seqs; s0 += kWave) {
-        const uint32_t s = s0 + lane_id();
-        bool le = false;
-        if (s < a.num_seqs) {
-            const uint64_t st = a.starts[s] < a.tokens ? a.starts[s] : a.tokens;
-            le = st * a.group / kRows + s <= tile;
-        }
-        const uint64_t m = __ballot(le);
-        before += (uint32_t)__popcll(m);
-        if (m != ~0ull) break;
-    }
-    if (before == 0) return t;
-    before = (uint32_t)__builtin_amdgcn_readfirstlane((int)before);
-    t.seq = before - 1;
+__device__ __forceinline__ AttItem att_item(const AttArgs& a, uint32_t item) {
+    AttItem t = {};
     const uint32_t lim = (uint32_t)a.tokens;
-    t.q0 = min(a.starts[t.seq], lim);
-    const uint32_t q1 = min(a.starts[t.seq + 1], lim);
-    if (q1 <= t.q0) return t;
-    t.q_len = q1 - t.q0;
-    const uint64_t rows = (uint64_t)t.q_len * a.group;
-    const uint64_t base = (uint64_t)t.q0 * a.group / kRows + t.seq;
-    const uint64_t first = (tile - base) * kRows;
-    if (first >= rows) return t;
-    const uint64_t cap = (uint64_t)a.max_pages << a.c.shift;
-    const uint32_t len = a.lens[t.seq];
-    t.kv_len = len < cap ? len : (uint32_t)cap;
-    if (a.c.num_pages == 0) t.kv_len = 0;
-    t.first = (uint32_t)first;
-    t.rows = (uint32_t)rows;
-    t.ok = true;
+    const uint32_t cap = a.c.num_pages ? a.max_pages << a.c.shift : 0;
+    uint32_t q0 = 0, len = 0, kv = 0;
+    auto read = [&](uint32_t s0) {
+        const uint32_t s = s0 + lane_id();
+        q0 = len = kv = 0;
+        if (s < a.num_seqs) {
+            q0 = min(a.starts[s], lim);
+            const uint32_t q1 = min(a.starts[s + 1], lim);
+            len = q1 > q0 ? q1 - q0 : 0;
+            kv = min(a.lens[s], cap);
+        }
+    };
+    auto tiles = [&] { return (len * a.group + kRows - 1) / kRows; };
+    t.chunk = 0xffffffffu;
+    if (a.target) {
+        // Sum over the sequences of f(tiles, steps).
+        const bool one = a.num_seqs <= kWave;
+        if (one) read(0);
+        auto sum = [&](auto f) {
+            uint64_t all = 0;
+            for (uint32_t s0 = 0; s0 < a.num_seqs; s0 += kWave) {
+                if (!one) read(s0);
+                all += f((uint64_t)tiles(), att_steps(kv));
+            }
+            const uint32_t lo = wave_total((uint32_t)all & 0xffffffu), hi = wave_total((uint32_t)(all >> 24));
+            return ((uint64_t)hi << 24) + lo;
+        };
+        const uint64_t all = sum([](uint64_t n, uint32_t steps) { return n * steps; });
+        uint64_t chunk = max((all + a.target - 1) / a.target, (uint64_t)kAttMinChunk);
+        // a chunk of all steps leaves a share a tile
+        while (chunk < kAttMaxSteps && sum([&](uint64_t n, uint32_t steps) {
+                   return n * max((steps + (uint32_t)chunk - 1) / (uint32_t)chunk, 1u);
+               }) > a.target)
+            chunk += (chunk + 7) / 8;
+        t.chunk = (uint32_t)min(chunk, (uint64_t)kAttMaxSteps);
+    }
+    uint32_t before = 0;  // items of the sequences gone by
+    for (uint32_t s0 = 0; s0 < a.num_seqs; s0 += kWave) {
+        if (!a.target || a.num_seqs > kWave) read(s0);  // else it has been
+        const uint32_t splits = a.target ? max((att_steps(kv) + t.chunk - 1) / t.chunk, 1u) : 1u;
+        const uint32_t count = tiles() * splits, sum = wave_scan(count);
+        const uint32_t all = (uint32_t)__builtin_amdgcn_readlane((int)sum, kWave - 1);
+        if (item - before >= all) {
+            before += all;
+            continue;
+        }
+        const int lane = (int)__popcll(__ballot(sum <= item - before));  // sequences that end before the item
+        t.seq = s0 + lane;
+        t.q0 = (uint32_t)__builtin_amdgcn_readlane((int)q0, lane);
+        t.q_len = (uint32_t)__builtin_amdgcn_readlane((int)len, lane);
+        t.kv_len = (uint32_t)__builtin_amdgcn_readlane((int)kv, lane);
+        t.splits = (uint32_t)__builtin_amdgcn_readlane((int)splits, lane);
+        const uint32_t n = (uint32_t)__builtin_amdgcn_readlane((int)count, lane);
+        const uint32_t at = item - before - ((uint32_t)__builtin_amdgcn_readlane((int)sum, lane) - n);
+        t.rows = t.q_len * a.group;
+        t.split = at % t.splits;
+        t.first = (n / t.splits - 1 - at / t.splits) * kRows;  // the rows that see the most keys first
+        t.ok = true;
+        return t;
+    }
     return t;
 }
 
 // Keys that row r of the sequence sees: all, or those up to its own position,
 // the last new token sitting at kv_len - 1.
-__device__ __forceinline__ uint32_t att_limit(const AttArgs& a, const AttTile& t, uint32_t r) {
+__device__ __forceinline__ uint32_t att_limit(const AttArgs& a, const AttItem& t, uint32_t r) {
     if (!a.causal) return t.kv_len;
     const uint32_t after = t.q_len - 1 - r / a.group;
     return t.kv_len > after ? t.kv_len - after : 0;
 }
-
-// Steps of a tile that sees `limit` keys, and their share for one split.
-__device__ __forceinline__ uint32_t att_steps(uint32_t limit) { return (limit + kAttStep - 1) / kAttStep; }
-__device__ __forceinline__ uint32_t att_share(uint32_t steps, uint32_t splits) { return (steps + splits - 1) / splits; }
 
 __device__ __forceinline__ uint32_t perm(uint32_t hi, uint32_t lo, uint32_t sel) {
     return __builtin_amdgcn_perm(hi, lo, sel);
@@ -144,53 +202,92 @@ __device__ __forceinline__ uint32_t pack_bf16(float x, float y, float* rx, float
     return u;
 }
 
+// Row r's query.
+__device__ __forceinline__ const float* att_query(const AttArgs& a, const AttItem& t, uint32_t head, uint32_t r) {
+    return a.q + (uint64_t)(t.q0 + r / a.group) * a.q_stride + (uint64_t)(head * a.group + r % a.group) * a.dim;
+}
+
 // What a lane loads of one 16-token tile.
 template <int NB>
 struct AttKV {
-    static constexpr int kV = NB < 4 ? 4 : NB;
-    uint32_t k[NB];  // token n's codes of group g, eight dimensions a dword
-    uint32_t v[kV];  // four tokens of chunk n (or half of n / 2, or 2n and 2n + 1)
-    uint32_t ks;     // K's scale bytes: one block's, or two blocks'
-    uint32_t vs;     // V's scale bytes of tokens 4g .. 4g + 3
-    uint32_t valid;  // tokens of the tile that exist
+    static constexpr int kC = NB < 4 ? 1 : NB / 4;  // 16-byte pieces
+    uint32_t k[NB];   // token n's codes of group g, eight dimensions a dword
+    u32x4 v[kC];      // four tokens of chunk n (or n / 2, or 2n and 2n + 1)
+    uint32_t ks[kC];  // K's scale bytes
+    uint32_t vs;      // V's scale bytes of tokens 4g .. 4g + 3
+    uint32_t valid;   // tokens of the tile that exist
 };
 
+// A value that the compiler takes as new, so that 32-bit offsets stay 32 bits wide
+// beside their use (a load from a scalar base) and no 64-bit sums are kept.
+__device__ __forceinline__ uint32_t opaque(uint32_t v) {
+    asm("" : "+v"(v));
+    return v;
+}
+
+// Adds v of the lanes N places round in each row of 16.
+template <int N>
+__device__ __forceinline__ float add_ror(float v) {
+    return v + __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0x120 + N, 0xf, 0xf, true));
+}
+
 // NB: blocks of 32 dimensions that the tiles hold (2, 4 or 8), nb <= NB of them
-// in use; R: 16-row tiles of a wave; Split: the workgroup's waves share the
-// rows and deal out the tokens, else each wave has rows of its own.
-template <int NB, int R, bool Split>
-__global__ __launch_bounds__(kAttBlock) void att_kernel(AttArgs a) {
-    constexpr uint32_t kRows = 16u * R * (Split ? 1 : kAttWaves);
-    constexpr int kJ = 2 * NB;                 // dimensions of a lane's O rows, O tiles
-    constexpr int kV = AttKV<NB>::kV;
+// in use.  kSlot: query rows of a matrix tile's 16 columns.  16: a product for
+// each of q's three terms and each of p's two.  With 8 or 4 rows (a decode step's
+// query heads) the terms lie side by side in the columns instead, column = slot *
+// kSlot + row: one product takes two or all three of q's terms and both of p's,
+// and the slots' scores are added across lanes.
+// R: 16-row tiles of a wave.  An item's rows are kSlot, or 64 R: its waves deal
+// out the rows, and where there are too few rows for four waves, the tokens,
+// whose parts they join at the end.
+template <int NB, int R, int kSlot>
+struct AttShape {
+    static constexpr uint32_t kWaveRows = kSlot < 16 ? kSlot : 16 * R;
+    static constexpr uint32_t kRows = kSlot < 16 ? kSlot : 16 * R * kAttWaves;
+    static constexpr int kSide = 16 / kSlot;                      // terms side by side
+    static constexpr int kQ = (kAttTerms + kSide - 1) / kSide;    // products for a score
+    static constexpr int kP = kSlot == 16 ? 2 : 1;                // products for an output
+};
+
+template <int NB, int R, int kSlot, int kPerSimd>
+__global__ __launch_bounds__(kAttBlock) __attribute__((amdgpu_waves_per_eu(kPerSimd, kPerSimd)))
+void att_kernel(AttArgs a) {
+    using Shape = AttShape<NB, R, kSlot>;
+    constexpr uint32_t kRows = Shape::kRows, kWaveRows = Shape::kWaveRows;
+    constexpr int kQ = Shape::kQ, kP = Shape::kP, kC = AttKV<NB>::kC;
+    constexpr int kJ = 2 * NB;  // dimensions of a lane's part of a row, and O tiles
     const uint32_t lane = threadIdx.x % kWave, n = lane % 16, g = lane / 16;
     const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x / kWave));
-    const uint32_t tile_id = a.tiles - 1 - a.tile0 - blockIdx.x;  // rows that see the most keys first
-    const uint32_t head = blockIdx.y, split = blockIdx.z;
-    const AttTile t = att_tile<kRows>(a, tile_id);
+    // Key heads change fastest: workgroups go round the 8 XCDs, and every XCD gets
+    // its part of the items, of which the last may be empty.
+    const uint32_t head = blockIdx.x % a.c.kv_heads, item = a.item0 + blockIdx.x / a.c.kv_heads;
+    const AttItem t = att_item<kRows>(a, item);
     if (!t.ok) return;
     const uint32_t nb = a.c.nb;
-    const uint32_t r0 = t.first + (Split ? 0 : wave * 16 * R);  // the wave's first row
+    // The waves' rows: one, two or four groups of them; the waves of a group share
+    // its tokens.
+    const uint32_t left = min(t.rows - t.first, kRows);
+    const uint32_t groups = left <= kWaveRows ? 1 : left <= 2 * kWaveRows ? 2 : 4;
+    const uint32_t share_of = kAttWaves / groups, part = wave / groups;
+    const uint32_t r0 = t.first + (wave % groups) * kWaveRows;  // the wave's first row
+    const uint32_t r1 = min(r0 + kWaveRows, t.rows);            // its end; r0 or less: no rows
     const uint32_t last_row = min(t.first + kRows, t.rows) - 1;
-    const bool have = r0 < t.rows;
 
     // Tokens of this split, then of this wave.
-    const uint32_t steps = att_steps(att_limit(a, t, last_row)), share = att_share(steps, a.splits);
-    const uint32_t lo = split * share, hi = min(lo + share, steps);
-    if (a.splits > 1 && lo >= hi) return;  // the joining kernel knows
-    uint32_t end = hi;
+    const uint32_t steps = att_steps(att_limit(a, t, last_row));
+    const uint32_t lo = t.splits > 1 ? t.split * t.chunk : 0, hi = t.splits > 1 ? min(lo + t.chunk, steps) : steps;
+    if (t.splits > 1 && lo >= hi) return;  // the joining kernel knows
     const uint32_t min_limit = att_limit(a, t, min(r0, t.rows - 1));
-    if (!Split) end = have ? min(hi, att_steps(att_limit(a, t, min(r0 + 16 * R, t.rows) - 1))) : 0;
+    const uint32_t end = r0 < r1 ? min(hi, att_steps(att_limit(a, t, r1 - 1))) : 0;
 
     uint32_t limit[R];
-    u32x4 qf[R][3][NB];
+    u32x4 qf[R][kQ][NB];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-        const uint32_t row = r0 + 16 * r + n;
-        const bool live = row < t.rows;
+        const uint32_t row = r0 + 16 * r + n % kSlot, slot = n / kSlot;
+        const bool live = row < r1;
         limit[r] = live ? att_limit(a, t, row) : 0;
-        const uint32_t tok = live ? t.q0 + row / a.group : 0, hd = head * a.group + row % a.group;
-        const float* qp = a.q + (uint64_t)tok * a.q_stride + (uint64_t)hd * a.dim;
+        const float* qp = att_query(a, t, head, live ? row : 0);
 #pragma unroll
         for (int j = 0; j < NB; ++j) {
             const uint32_t d0 = g * 8 * NB + 8 * j;
@@ -210,12 +307,21 @@ __global__ __launch_bounds__(kAttBlock) void att_kernel(AttArgs a) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 float u = x[2 * i] * a.scale_log2, v = x[2 * i + 1] * a.scale_log2;
+                uint32_t term[kAttTerms];
 #pragma unroll
-                for (int term = 0; term < 3; ++term) {  // the top 16 bits, then what they leave
+                for (int k = 0; k < kAttTerms; ++k) {  // the top 16 bits, then what they leave
                     const uint32_t ub = __float_as_uint(u), vb = __float_as_uint(v);
-                    qf[r][term][j][i] = perm(vb, ub, 0x07060302u);
+                    term[k] = perm(vb, ub, 0x07060302u);
                     u -= __uint_as_float(ub & 0xffff0000u);
                     v -= __uint_as_float(vb & 0xffff0000u);
+                }
+#pragma unroll
+                for (int k = 0; k < kQ; ++k) {
+                    uint32_t w = 0;
+#pragma unroll
+                    for (int at = 0; at < Shape::kSide; ++at)
+                        if (k * Shape::kSide + at < kAttTerms && slot == (uint32_t)at) w = term[k * Shape::kSide + at];
+                    qf[r][k][j][i] = w;
                 }
             }
         }
@@ -233,98 +339,78 @@ __global__ __launch_bounds__(kAttBlock) void att_kernel(AttArgs a) {
         for (int j = 0; j < kJ; ++j) o[r][j] = zero;
     }
 
-    const uint32_t* table = a.table + (uint64_t)t.seq * a.max_pages;
-    // Tile tt's place in the cache; a page that does not exist has no tokens.
-    auto place = [&](uint32_t tt, uint32_t* valid) {
-        const uint32_t at = tt * 16;
-        uint32_t page = 0, v = 0;
-        if (at < t.kv_len) {
-            page = (uint32_t)__builtin_amdgcn_readfirstlane((int)table[at >> a.c.shift]);
-            v = min(t.kv_len - at, 16u);
-            if (page >= a.c.num_pages) page = 0, v = 0;
-        }
-        *valid = v;
-        return a.cache + (uint64_t)page * a.c.page_bytes + (uint64_t)head * a.c.head_bytes;
-    };
-    auto load = [&](uint32_t tt, AttKV<NB>& x) {
-        const uint8_t* base = place(tt, &x.valid);
-        const uint32_t t0 = (tt * 16) & (a.c.page - 1), np = a.c.page * nb;
-        const uint8_t* kp = base + (t0 + n) * nb * 16 + g * 4 * NB;
-        const uint8_t* vp = base + np * 16 + t0 * nb * 16;
-        const uint8_t* ksp = base + np * 32 + (t0 + n) * nb;
-        const uint8_t* vsp = base + np * 33 + t0 * nb + 4 * g;
-        x.ks = x.vs = 0x7f7f7f7fu;
+    // Loads have no conditions on their way, so that a step's can be waited for
+    // while the next one's are in flight: a tile past the end is one of page 0 with
+    // no tokens, blocks past nb are read from the last one (q is zero there, and
+    // what they add to the output is not stored).
+    typedef const __attribute__((address_space(4))) uint32_t* ScalarPtr;
+    const ScalarPtr table = (ScalarPtr)(uintptr_t)(a.table + (uint64_t)t.seq * a.max_pages);
+    const uint32_t last_page = t.kv_len ? (t.kv_len - 1) >> a.c.shift : 0;
+    auto page_of = [&](uint32_t tt) { return table[min(tt * 16 >> a.c.shift, last_page)]; };
+    const uint32_t stride = share_of;
+    uint32_t koff[kC], ksoff[kC], voff[kC], vsoff = 0;
 #pragma unroll
-        for (int j = 0; j < NB; ++j) x.k[j] = 0;
+    for (int c = 0; c < kC; ++c) {
+        const uint32_t np = a.c.page * nb, kb = min(NB == 2 ? g / 2 : g * kC + c, nb - 1);
+        koff[c] = n * nb * 16 + kb * 16 + (NB == 2 ? g % 2 * 8 : 0);
+        ksoff[c] = np * 32 + n * nb + kb;
+        const uint32_t chunk = min(NB == 2 ? n / 2 : n * kC + c, 4 * nb - 1);
+        voff[c] = np * 16 + (g * 4 * nb + chunk) * 16;
+        if (c == 0) vsoff = np * 33 + chunk / 4 * 16 + 4 * g;
+    }
+    auto load = [&](uint32_t tt, uint32_t page, AttKV<NB>& x) {
+        x.valid = min(t.kv_len - min(t.kv_len, tt * 16), 16u);
+        if (page >= a.c.num_pages) page = 0, x.valid = 0;  // a page that does not exist has no tokens
+        const uint32_t t0 = (tt * 16) & (a.c.page - 1);
+        const uint8_t* base = a.cache + (uint64_t)page * a.c.page_bytes + (uint64_t)head * a.c.head_bytes;
+        const uint8_t* codes = base + t0 * nb * 16;
+        const uint8_t* scales = base + t0 * nb;
 #pragma unroll
-        for (int j = 0; j < kV; ++j) x.v[j] = 0;
-        if constexpr (NB == 2) {
-            if (g < 2 * nb) {
-                const u32x2 u = *reinterpret_cast<const u32x2*>(kp);
+        for (int c = 0; c < kC; ++c) {
+            if constexpr (NB == 2) {
+                const u32x2 u = *reinterpret_cast<const u32x2*>(codes + opaque(koff[c]));
                 x.k[0] = u.x;
                 x.k[1] = u.y;
-                x.ks = ksp[g >> 1];
+            } else {
+                const u32x4 u = *reinterpret_cast<const u32x4*>(codes + opaque(koff[c]));
+#pragma unroll
+                for (int i = 0; i < 4; ++i) x.k[4 * c + i] = u[i];
             }
-            if (n >> 1 < 4 * nb) {
-                const u32x4 u = *reinterpret_cast<const u32x4*>(vp + (g * 4 * nb + (n >> 1)) * 16);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) x.v[i] = u[i] >> (n & 1) * 16;  // the lane's four dimensions
-                x.vs = *reinterpret_cast<const uint32_t*>(vsp + (n >> 3) * 16);
-            }
-        } else {
-#pragma unroll
-            for (int c = 0; c < NB / 4; ++c) {
-                const uint32_t block = g * (NB / 4) + c;
-                if (block < nb) {
-                    const u32x4 u = *reinterpret_cast<const u32x4*>(kp + 16 * c);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) x.k[4 * c + i] = u[i];
-                    x.ks = c ? (x.ks & 0xffu) | (uint32_t)ksp[block] << 8 : ksp[block];
-                }
-                const uint32_t chunk = n * (NB / 4) + c;
-                if (chunk < 4 * nb) {
-                    const u32x4 u = *reinterpret_cast<const u32x4*>(vp + (g * 4 * nb + chunk) * 16);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) x.v[4 * c + i] = u[i];
-                    if (c == 0) x.vs = *reinterpret_cast<const uint32_t*>(vsp + (chunk >> 2) * 16);
-                }
-            }
+            x.v[c] = *reinterpret_cast<const u32x4*>(codes + opaque(voff[c]));
+            x.ks[c] = scales[opaque(ksoff[c])];
         }
+        x.vs = *reinterpret_cast<const uint32_t*>(scales + opaque(vsoff));
     };
 
-    const uint32_t stride = Split ? kAttWaves : 1;
-    AttKV<NB> cur[2], nxt[2];
-    uint32_t step = lo + (Split ? wave : 0);
-    if (step < end) {
-        load(2 * step, cur[0]);
-        load(2 * step + 1, cur[1]);
-    }
-    for (; step < end; step += stride) {
-        if (step + stride < end) {
-            load(2 * (step + stride), nxt[0]);
-            load(2 * (step + stride) + 1, nxt[1]);
-        }
+    auto work = [&](uint32_t step, AttKV<NB> (&cur)[2], uint32_t page0, uint32_t page1) {
         // Scores: tokens 4g + i of both tiles, in powers of two.
         f32x4 s[R][2];
 #pragma unroll
-        for (int x = 0; x < 2; ++x) {
+        for (int r = 0; r < R; ++r) s[r][0] = s[r][1] = zero;
 #pragma unroll
-            for (int r = 0; r < R; ++r) s[r][x] = zero;
+        for (int j = 0; j < NB; ++j)
 #pragma unroll
-            for (int j = 0; j < NB; ++j) {
-                const uint32_t b = NB == 8 && j >= 4 ? cur[x].ks >> 8 : cur[x].ks & 0xffu;
-                const float sc = __uint_as_float(b << 23);
-                const u32x4 kf = {cvt2<0>(cur[x].k[j], sc), cvt2<1>(cur[x].k[j], sc), cvt2<2>(cur[x].k[j], sc),
-                                  cvt2<3>(cur[x].k[j], sc)};
+            for (int x = 0; x < 2; ++x) {
+                const float sc = __uint_as_float(cur[x].ks[j / 4] << 23);
+                const uint32_t code = cur[x].k[j];
+                const u32x4 kf = {cvt2<0>(code, sc), cvt2<1>(code, sc), cvt2<2>(code, sc), cvt2<3>(code, sc)};
 #pragma unroll
-                for (int r = 0; r < R; ++r)
+                for (int k = kQ - 1; k >= 0; --k)
 #pragma unroll
-                    for (int term = 2; term >= 0; --term) s[r][x] = mfma(kf, qf[r][term][j], s[r][x]);
+                    for (int r = 0; r < R; ++r) s[r][x] = mfma(kf, qf[r][k][j], s[r][x]);
             }
+        if constexpr (kSlot < 16) {
+#pragma unroll
+            for (int x = 0; x < 2; ++x)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    s[0][x][i] = add_ror<8>(s[0][x][i]);
+                    if constexpr (kSlot == 4) s[0][x][i] = add_ror<4>(s[0][x][i]);
+                }
         }
         const uint32_t at = step * kAttStep;
         // Every row of the wave sees every token of the step: no masks.
-        const bool whole = at + kAttStep <= min_limit && cur[0].valid == 16 && cur[1].valid == 16;
+        const bool whole = at + kAttStep <= min_limit && cur[0].valid + cur[1].valid == kAttStep;
         bool nan_v = false;
         if (!whole) {
 #pragma unroll
@@ -346,15 +432,15 @@ __global__ __launch_bounds__(kAttBlock) void att_kernel(AttArgs a) {
                 cur[x].vs = vs;
             }
         }
-        // Running maximum, probabilities and their sum; two bf16 terms.
-        u32x4 pf[R][2];
+        // Running maximum, probabilities and their sum; bf16 terms.
+        u32x4 pf[R][kP];
 #pragma unroll
         for (int r = 0; r < R; ++r) {
             float mx = fmaxf(fmaxf(fmaxf(s[r][0][0], s[r][0][1]), fmaxf(s[r][0][2], s[r][0][3])),
                              fmaxf(fmaxf(s[r][1][0], s[r][1][1]), fmaxf(s[r][1][2], s[r][1][3])));
-            mx = fmaxf(mx, __shfl_xor(mx, 16, kWave));
-            mx = fmaxf(mx, __shfl_xor(mx, 32, kWave));
             if (__any(mx > m[r])) {
+                mx = fmaxf(mx, __shfl_xor(mx, 16, kWave));
+                mx = fmaxf(mx, __shfl_xor(mx, 32, kWave));
                 const float mn = fmaxf(m[r], mx);
                 const float f = mn > m[r] ? __builtin_amdgcn_exp2f(m[r] - mn) : 1.0f;
                 m[r] = mn;
@@ -367,12 +453,17 @@ __global__ __launch_bounds__(kAttBlock) void att_kernel(AttArgs a) {
             for (int x = 0; x < 2; ++x)
 #pragma unroll
                 for (int i = 0; i < 4; i += 2) {
-                    const float p0 = __builtin_amdgcn_exp2f(s[r][x][i] - base);
-                    const float p1 = __builtin_amdgcn_exp2f(s[r][x][i + 1] - base);
+                    float p0 = __builtin_amdgcn_exp2f(s[r][x][i] - base);
+                    float p1 = __builtin_amdgcn_exp2f(s[r][x][i + 1] - base);
                     l[r] += p0 + p1;
                     float e0, e1, u0, u1;
-                    pf[r][0][2 * x + i / 2] = pack_bf16(p0, p1, &e0, &e1);
-                    pf[r][1][2 * x + i / 2] = pack_bf16(e0, e1, &u0, &u1);
+                    const uint32_t top = pack_bf16(p0, p1, &e0, &e1);
+                    if constexpr (kSlot == 16) {
+                        pf[r][0][2 * x + i / 2] = top;
+                        pf[r][1][2 * x + i / 2] = pack_bf16(e0, e1, &u0, &u1);
+                    } else {  // slot 0 holds the first term, slot 1 the second; the others are not read
+                        pf[r][0][2 * x + i / 2] = n < kSlot ? top : pack_bf16(e0, e1, &u0, &u1);
+                    }
                 }
         }
         // V: four dwords a tile are four tokens x eight dimensions; an operand is
@@ -385,7 +476,8 @@ __global__ __launch_bounds__(kAttBlock) void att_kernel(AttArgs a) {
             uint32_t v[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const uint32_t code = cur[i >> 2].v[(NB == 8 ? (p >> 2) * 4 : 0) + (i & 3)];
+                uint32_t code = cur[i >> 2].v[NB == 8 ? p >> 2 : 0][i & 3];
+                if (NB == 2) code >>= (n & 1) * 16;  // the lane's four dimensions of the chunk
                 v[i] = (p & 3) == 0   ? cvt2<0>(code, vsc[i])
                        : (p & 3) == 1 ? cvt2<1>(code, vsc[i])
                        : (p & 3) == 2 ? cvt2<2>(code, vsc[i])
@@ -397,19 +489,18 @@ __global__ __launch_bounds__(kAttBlock) void att_kernel(AttArgs a) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) vf[i] = perm(v[2 * i + 1], v[2 * i], h ? 0x07060302u : 0x05040100u);
 #pragma unroll
-                for (int r = 0; r < R; ++r) {
-                    o[r][2 * p + h] = mfma(vf, pf[r][1], o[r][2 * p + h]);
-                    o[r][2 * p + h] = mfma(vf, pf[r][0], o[r][2 * p + h]);
-                }
+                for (int k = kP - 1; k >= 0; --k)
+#pragma unroll
+                    for (int r = 0; r < R; ++r) o[r][2 * p + h] = mfma(vf, pf[r][k], o[r][2 * p + h]);
             }
         }
         // A NaN block of a token that some rows do not see: its 32 dimensions of
         // the rows that do.
         if (!whole && __any(nan_v)) {
             for (uint32_t x = 0; x < 2; ++x) {
-                uint32_t valid;
-                const uint8_t* base = place(2 * step + x, &valid);
-                const uint32_t t0 = (at + 16 * x) & (a.c.page - 1);
+                const uint32_t page = x ? page1 : page0, t0 = (at + 16 * x) & (a.c.page - 1);
+                const uint32_t valid = x ? cur[1].valid : cur[0].valid;
+                const uint8_t* base = a.cache + (uint64_t)page * a.c.page_bytes + (uint64_t)head * a.c.head_bytes;
                 for (uint32_t b = 0; b < nb; ++b)
                     for (uint32_t i = 0; i < valid; ++i)
                         if (base[q4_v_scale(a.c, t0 + i, b)] == kQ4NanScale)
@@ -423,8 +514,36 @@ __global__ __launch_bounds__(kAttBlock) void att_kernel(AttArgs a) {
                                             for (int j = 0; j < kJ; ++j) o[r][j][k] = __uint_as_float(0x7fc00000u);
             }
         }
-        cur[0] = nxt[0];
-        cur[1] = nxt[1];
+    };
+
+    // Two steps in turn: one's loads are in flight while the other is worked on,
+    // the pages of the one after that on their way.
+    uint32_t step = lo + part;
+    if (step < end) {
+        AttKV<NB> kv[2][2];
+        uint32_t pg[2][2], ahead[2];
+        auto fetch = [&](uint32_t st, int to) {
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                pg[to][x] = ahead[x];
+                load(2 * st + x, ahead[x], kv[to][x]);
+            }
+#pragma unroll
+            for (int x = 0; x < 2; ++x) ahead[x] = page_of(2 * (st + stride) + x);
+        };
+        ahead[0] = page_of(2 * step);
+        ahead[1] = page_of(2 * step + 1);
+        fetch(step, 0);
+        for (;;) {
+            fetch(step + stride, 1);
+            work(step, kv[0], pg[0][0], pg[0][1]);
+            step += stride;
+            if (step >= end) break;
+            fetch(step + stride, 0);
+            work(step, kv[1], pg[1][0], pg[1][1]);
+            step += stride;
+            if (step >= end) break;
+        }
     }
 
 #pragma unroll
@@ -433,135 +552,182 @@ __global__ __launch_bounds__(kAttBlock) void att_kernel(AttArgs a) {
         l[r] += __shfl_xor(l[r], 32, kWave);
     }
     // Lane (n, g) has dimensions kJ (4g + i) + j of row n in o[.][j][i].
-    const uint64_t part0 = (((uint64_t)tile_id * a.c.kv_heads + head) * a.splits + split) * kRows;
+    const uint64_t part0 = ((uint64_t)item * a.c.kv_heads + head) * kRows;
     const uint32_t dp = 32 * nb;
     float* const pm = a.part;  // [rows][2] of all, then [rows][dp] of all
-    float* const po = a.part + (uint64_t)a.tiles * a.c.kv_heads * a.splits * kRows * 2;
-    auto store_row = [&](uint32_t row, float mm, float ll, uint32_t d, const float* v, int count) {
-        // `count` values from dimension d of row `row` of the tile, not yet divided
-        const uint32_t rr = t.first + row;
-        if (rr >= t.rows) return;
-        if (a.splits > 1) {
+    float* const po = a.part + (uint64_t)a.items * a.c.kv_heads * kRows * 2;
+    // `count` values from dimension d of the sequence's row rr, not yet divided.
+    auto store_row = [&](uint32_t rr, float mm, float ll, uint32_t d, const float* v, auto count) {
+        constexpr int kCount = decltype(count)::value;
+        if (t.splits > 1) {
+            const uint64_t at = part0 + (rr - t.first);
             if (d == 0) {
-                pm[(part0 + row) * 2] = mm;
-                pm[(part0 + row) * 2 + 1] = ll;
+                pm[at * 2] = mm;
+                pm[at * 2 + 1] = ll;
             }
-            float* p = po + (part0 + row) * dp + d;
+            float* p = po + at * dp + d;
 #pragma unroll
-            for (int i = 0; i < count; ++i)
-                if (d + i < dp) p[i] = v[i];
+            for (int i = 0; i < kCount; i += 4)
+                if (d + i < dp) *reinterpret_cast<f32x4*>(p + i) = {v[i], v[i + 1], v[i + 2], v[i + 3]};
         } else {
             const float f = ll == 0.0f ? 0.0f : 1.0f / ll;
             float* p = a.out + ((uint64_t)(t.q0 + rr / a.group) * a.q_heads + head * a.group + rr % a.group) * a.dim + d;
 #pragma unroll
-            for (int i = 0; i < count; ++i)
-                if (d + i < a.dim) p[i] = ll == 0.0f ? 0.0f : v[i] * f;
+            for (int i = 0; i < kCount; i += 4) {
+                float u[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) u[k] = ll == 0.0f ? 0.0f : v[i + k] * f;
+                if (d + i + 4 <= a.dim) {
+                    *reinterpret_cast<f32x4_a4*>(p + i) = {u[0], u[1], u[2], u[3]};
+                } else {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        if (d + i + k < a.dim) p[i + k] = u[k];
+                }
+            }
         }
     };
-    if constexpr (!Split) {
+    if (groups == kAttWaves) {
+        if constexpr (kSlot == 16) {
 #pragma unroll
-        for (int r = 0; r < R; ++r)
+            for (int r = 0; r < R; ++r) {
+                const uint32_t row = r0 + 16 * r + n;
+                if (row >= r1) continue;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                float v[kJ];
+                for (int i = 0; i < 4; ++i) {
+                    float v[kJ];
 #pragma unroll
-                for (int j = 0; j < kJ; ++j) v[j] = o[r][j][i];
-                store_row(wave * 16 * R + 16 * r + n, m[r], l[r], kJ * (4 * g + i), v, kJ);
-            }
-    } else {
-        // Join the waves: to the common maximum, then add.
-        constexpr int kPitch = 16 * kJ + 4;
-        __shared__ float sm[kAttWaves][16], sl[kAttWaves][16];
-        __shared__ __attribute__((aligned(16))) float so[kAttWaves][16][kPitch];
-#pragma unroll
-        for (int r = 0; r < R; ++r) {
-            __syncthreads();
-            if (g == 0) {
-                sm[wave][n] = m[r];
-                sl[wave][n] = l[r];
-            }
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int j = 0; j < kJ; ++j) so[wave][n][kJ * (4 * g + i) + j] = o[r][j][i];
-            __syncthreads();
-            const uint32_t row = threadIdx.x / 16;
-            float mm = ninf, ll = 0.0f, f[kAttWaves];
-#pragma unroll
-            for (int w = 0; w < kAttWaves; ++w) mm = fmaxf(mm, sm[w][row]);
-#pragma unroll
-            for (int w = 0; w < kAttWaves; ++w) {
-                // a wave that saw nothing holds zeros (or NaN, which stays)
-                f[w] = sm[w][row] == ninf ? 1.0f : __builtin_amdgcn_exp2f(sm[w][row] - mm);
-                ll += sl[w][row] * f[w];
-            }
-            for (uint32_t d = (threadIdx.x % 16) * 4; d < (uint32_t)(16 * kJ); d += 64) {
-                float v[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int w = 0; w < kAttWaves; ++w) {
-                    const f32x4 u = *reinterpret_cast<const f32x4*>(&so[w][row][d]);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) v[i] += u[i] * f[w];
+                    for (int j = 0; j < kJ; ++j) v[j] = o[r][j][i];
+                    store_row(row, m[r], l[r], kJ * (4 * g + i), v, std::integral_constant<int, kJ>());
                 }
-                store_row(16 * r + row, mm, ll, d, v, 4);
             }
         }
+        return;
     }
-}
-
-// Joins a tile's splits.
-template <uint32_t kRows>
-__global__ __launch_bounds__(kAttCombine) void att_combine_kernel(AttArgs a) {
-    const uint32_t head = blockIdx.y;
-    const uint32_t tile_id = a.tile0 + blockIdx.x;
-    const AttTile t = att_tile<kRows>(a, tile_id);
-    if (!t.ok) return;
-    const uint32_t last_row = min(t.first + kRows, t.rows) - 1;
-    const uint32_t steps = att_steps(att_limit(a, t, last_row)), share = att_share(steps, a.splits);
-    const uint32_t used = steps ? (steps + share - 1) / share : 0;
-    const uint64_t part0 = ((uint64_t)tile_id * a.c.kv_heads + head) * a.splits * kRows;
-    const float* pm = a.part;
-    const float* po = a.part + (uint64_t)a.tiles * a.c.kv_heads * a.splits * kRows * 2;
-    const uint32_t dp = 32 * a.c.nb, per_row = dp / 4;
-    const float ninf = -__builtin_inff();
-    for (uint32_t i = threadIdx.x; i < kRows * per_row; i += kAttCombine) {
-        const uint32_t row = i / per_row, d = (i - row * per_row) * 4, rr = t.first + row;
-        if (rr >= t.rows) break;
-        float mm = ninf, ll = 0.0f;
-        for (uint32_t z = 0; z < used; ++z) mm = fmaxf(mm, pm[(part0 + z * kRows + row) * 2]);
-        f32x4 v = {0.f, 0.f, 0.f, 0.f};
-        for (uint32_t z = 0; z < used; ++z) {
-            const uint64_t at = part0 + z * kRows + row;
-            const float mz = pm[at * 2];
-            const float f = mz == ninf ? 1.0f : __builtin_amdgcn_exp2f(mz - mm);
-            ll += pm[at * 2 + 1] * f;
-            v += *reinterpret_cast<const f32x4*>(po + at * dp + d) * f;
-        }
-        float* p = a.out + ((uint64_t)(t.q0 + rr / a.group) * a.q_heads + head * a.group + rr % a.group) * a.dim;
-        const float f = 1.0f / ll;
+    // Join the waves of a group: to the common maximum, then add (and the second
+    // term's column to the first's).
+    constexpr int kPitch = 16 * kJ + 4;
+    __shared__ float sm[kAttWaves][16], sl[kAttWaves][16];
+    __shared__ __attribute__((aligned(16))) float so[kAttWaves][16][kPitch];
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
-            if (d + k < a.dim) p[d + k] = ll == 0.0f ? 0.0f : v[k] * f;
+    for (int r = 0; r < R; ++r) {
+        __syncthreads();
+        if (g == 0) {
+            sm[wave][n] = m[r];
+            sl[wave][n] = l[r];
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < kJ; j += 4)
+                *reinterpret_cast<f32x4*>(&so[wave][n][kJ * (4 * g + i) + j]) = {o[r][j][i], o[r][j + 1][i],
+                                                                                o[r][j + 2][i], o[r][j + 3][i]};
+        __syncthreads();
+        constexpr uint32_t kTall = kSlot < 16 ? kSlot : 16;  // rows of one group's tile
+        constexpr uint32_t kQuads = 4 * kJ;                  // float4 of a row
+        for (uint32_t i = threadIdx.x; i < groups * kTall * kQuads; i += kAttBlock) {
+            const uint32_t d = i % kQuads * 4, row = i / kQuads % kTall, gr = i / kQuads / kTall;
+            const uint32_t rr = t.first + gr * kWaveRows + 16 * r + row;
+            if (rr >= t.rows) continue;
+            float mm = ninf, ll = 0.0f;
+            for (uint32_t w = gr; w < kAttWaves; w += groups) mm = fmaxf(mm, sm[w][row]);
+            float v[4] = {0.f, 0.f, 0.f, 0.f};
+            for (uint32_t w = gr; w < kAttWaves; w += groups) {
+                // a wave that saw nothing holds zeros (or NaN, which stays)
+                const float f = sm[w][row] == ninf ? 1.0f : __builtin_amdgcn_exp2f(sm[w][row] - mm);
+                ll += sl[w][row] * f;
+                f32x4 u = *reinterpret_cast<const f32x4*>(&so[w][row][d]);
+                if (kSlot < 16) u += *reinterpret_cast<const f32x4*>(&so[w][row + kSlot % 16][d]);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) v[k] += u[k] * f;
+            }
+            store_row(rr, mm, ll, d, v, std::integral_constant<int, 4>());
+        }
     }
 }
 
+// Joins the shares of a tile, kJoinRows rows at a time: their maxima and sums
+// through LDS, then a thread has four dimensions of a row and every kth share.
+constexpr uint32_t kJoinRows = 4;
+
+template <uint32_t kRows>
+__global__ __launch_bounds__(kAttJoin) void att_join_kernel(AttArgs a) {
+    __shared__ float2 ml[kJoinRows][kAttMaxSplits];
+    __shared__ f32x4 red[kAttJoin];
+    const uint32_t head = blockIdx.x % a.c.kv_heads, item = a.item0 + blockIdx.x / a.c.kv_heads;
+    const AttItem t = att_item<kRows>(a, item);
+    if (!t.ok || t.split || t.splits == 1) return;
+    const uint32_t last_row = min(t.first + kRows, t.rows) - 1;
+    const uint32_t used = (att_steps(att_limit(a, t, last_row)) + t.chunk - 1) / t.chunk;
+    const uint64_t next = (uint64_t)a.c.kv_heads * kRows;  // rows to the next share's
+    const float* po = a.part + (uint64_t)a.items * a.c.kv_heads * kRows * 2;
+    const uint32_t dp = 32 * a.c.nb, quads = dp / 4, group = kJoinRows * quads, groups = kAttJoin / group;
+    const uint32_t gr = threadIdx.x / group, row = threadIdx.x % group / quads, d = threadIdx.x % quads * 4;
+    for (uint32_t row0 = 0; row0 < kRows && t.first + row0 < t.rows; row0 += kJoinRows) {
+        const uint64_t part0 = ((uint64_t)item * a.c.kv_heads + head) * kRows + row0;
+        const float2* pm = reinterpret_cast<const float2*>(a.part) + part0;
+        __syncthreads();
+        // rows past the sequence's hold anything and are not stored
+        for (uint32_t i = threadIdx.x; i < used * kJoinRows; i += kAttJoin)
+            ml[i % kJoinRows][i / kJoinRows] = pm[i / kJoinRows * next + i % kJoinRows];
+        __syncthreads();
+        const float ninf = -__builtin_inff();
+        float mm = ninf, ll = 0.0f;
+        f32x4 v = {0.f, 0.f, 0.f, 0.f};
+        if (gr < groups) {
+            for (uint32_t z = 0; z < used; ++z) mm = fmaxf(mm, ml[row][z].x);
+            const float* p = po + (part0 + row) * dp + d;
+#pragma unroll 8
+            for (uint32_t z = gr; z < used; z += groups) {
+                const float2 u = ml[row][z];
+                // a share that saw nothing holds zeros (or NaN, which stays)
+                const float f = u.x == ninf ? 1.0f : __builtin_amdgcn_exp2f(u.x - mm);
+                v += *reinterpret_cast<const f32x4*>(p + z * next * dp) * f;
+            }
+        }
+        red[threadIdx.x] = v;
+        __syncthreads();
+        const uint32_t rr = t.first + row0 + row;
+        if (gr == 0 && rr < t.rows) {
+            for (uint32_t k = 1; k < groups; ++k) v += red[threadIdx.x + k * group];
+            for (uint32_t z = 0; z < used; ++z) {
+                const float2 u = ml[row][z];
+                ll += u.x == ninf ? u.y : u.y * __builtin_amdgcn_exp2f(u.x - mm);
+            }
+            float* out = a.out + ((uint64_t)(t.q0 + rr / a.group) * a.q_heads + head * a.group + rr % a.group) * a.dim;
+            const float f = 1.0f / ll;
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                if (d + k < a.dim) out[d + k] = ll == 0.0f ? 0.0f : v[k] * f;
+        }
+    }
+}
+
+// Rows of an item: a decode step's query heads in a few columns, or rows for four
+// waves.
 struct AttPlan {
-    uint32_t rows;  // rows of a workgroup's tile
-    uint32_t tiles, splits;
+    int slot, r;    // kSlot, R
+    uint32_t rows;  // kRows
+    uint32_t items, target;
     uint64_t bytes;  // workspace
 };
 
 static int att_plan(uint64_t num_seqs, uint64_t tokens, uint64_t q_heads, uint64_t kv_heads, uint64_t page_size,
                     uint64_t max_pages, uint32_t nb, AttPlan* p) {
-    const uint64_t group = q_heads / kv_heads;
-    p->rows = 16;
-    const uint64_t tiles = tokens * group / p->rows + num_seqs;
+    const uint64_t group = q_heads / kv_heads, rows = tokens * group;
+    p->slot = rows <= 4 * num_seqs ? 4 : rows <= 8 * num_seqs ? 8 : 16;
+    p->r = p->slot < 16 || nb > 4 ? 1 : 2;
+    p->rows = p->slot < 16 ? p->slot : 64u * p->r;
+    const uint64_t tiles = rows / p->rows + num_seqs;
     if (tiles > 0x3fffffull) return KORE_HIP_ERR_OVERFLOW;
-    p->tiles = (uint32_t)tiles;
-    const uint64_t busy = std::max<uint64_t>(1, std::max(std::min(num_seqs, tokens), tokens * group / p->rows)) * kv_heads;
-    const uint64_t cap = std::max<uint64_t>(1, max_pages * page_size / 256);
-    p->splits = (uint32_t)std::min<uint64_t>({(512 + busy - 1) / busy, cap, 1024});
-    p->bytes = p->splits > 1 ? tiles * kv_heads * p->splits * p->rows * (2 + 32ull * nb) * 4 : 0;
+    // Workgroups that the keys are cut for: what the chip holds at once.
+    const uint64_t want = p->slot == 4 && nb <= 4 ? 768 : 512;
+    const uint64_t busy = std::max(std::min(num_seqs, tokens), rows / p->rows) * kv_heads;
+    const uint64_t shares = max_pages * page_size / (kAttMinChunk * kAttStep);  // of the longest sequence
+    const bool cut = busy < (p->slot < 16 ? 2 * want : want / 2) && shares > 1;
+    p->target = cut ? (uint32_t)std::min<uint64_t>({(want + kv_heads - 1) / kv_heads, tiles * shares, kAttMaxSplits}) : 0;
+    p->items = std::max((uint32_t)tiles, p->target);
+    p->bytes = cut ? (uint64_t)p->items * kv_heads * p->rows * (2 + 32ull * nb) * 4 : 0;
     return KORE_HIP_OK;
 }
 
@@ -572,10 +738,31 @@ static int att_check(uint64_t num_seqs, uint64_t tokens, uint64_t q_heads, uint6
     if (st != KORE_HIP_OK) return st;
     if (kv_heads == 0 || q_heads % kv_heads) return KORE_HIP_ERR_BAD_DIM;
     if (num_seqs > 0x7fffffffull || tokens > 0x7fffffffull || q_heads > 65535u ||
-        max_pages > 0xffffffffull / page_size || (num_seqs && max_pages > kMaxElements / num_seqs) ||
+        max_pages > 0x7fffffffull / page_size || (num_seqs && max_pages > kMaxElements / num_seqs) ||
         tokens * q_heads > 0xffffffffull)
         return KORE_HIP_ERR_OVERFLOW;
     return att_plan(num_seqs, tokens, q_heads, kv_heads, page_size, max_pages, c->nb, p);
+}
+
+template <int NB, int R, int kSlot, int kPerSimd>
+static void att_launch_shape(const AttArgs& a, bool join, dim3 grid, hipStream_t s) {
+    if (join)
+        hipLaunchKernelGGL((att_join_kernel<AttShape<NB, R, kSlot>::kRows>), grid, dim3(kAttJoin), 0, s, a);
+    else
+        hipLaunchKernelGGL((att_kernel<NB, R, kSlot, kPerSimd>), grid, dim3(kAttBlock), 0, s, a);
+}
+
+static void att_launch(const AttArgs& a, const AttPlan& p, bool join, dim3 grid, hipStream_t s) {
+    const int nb = a.c.nb <= 2 ? 2 : a.c.nb <= 4 ? 4 : 8;
+    auto any = [&](auto blocks) {
+        constexpr int NB = decltype(blocks)::value;
+        if (p.slot == 4) att_launch_shape<NB, 1, 4, NB == 8 ? 2 : 3>(a, join, grid, s);
+        else if (p.slot == 8) att_launch_shape<NB, 1, 8, NB == 8 ? 1 : 2>(a, join, grid, s);
+        else att_launch_shape<NB, NB == 8 ? 1 : 2, 16, NB == 8 ? 1 : 2>(a, join, grid, s);
+    };
+    if (nb == 2) any(std::integral_constant<int, 2>());
+    else if (nb == 4) any(std::integral_constant<int, 4>());
+    else any(std::integral_constant<int, 8>());
 }
 
 static bool att_overlap(const void* a, uint64_t na, const void* b, uint64_t nb) {
@@ -639,27 +826,19 @@ extern "C" int kore_hip_attention_q4_f32(const float* q, const uint8_t* cache, c
     a.group = (uint32_t)(q_heads / kv_heads);
     a.max_pages = (uint32_t)max_pages;
     a.dim = (uint32_t)head_dim;
-    a.tiles = p.tiles;
-    a.splits = p.splits;
+    a.items = p.items;
+    a.target = p.target;
     a.scale_log2 = (float)((double)scale * 1.4426950408889634);
     a.causal = causal != 0;
-    hipStream_t s = (hipStream_t)stream;
-    // A launch holds fewer than 2^32 threads: tiles in bands.
-    const uint32_t band = (uint32_t)std::max<uint64_t>(1, 0x400000u / (kv_heads * p.splits));
-    for (a.tile0 = 0; a.tile0 < p.tiles; a.tile0 += band) {
-        const dim3 grid(std::min(band, p.tiles - a.tile0), (uint32_t)kv_heads, p.splits), block(kAttBlock);
-        if (a.c.nb <= 2) hipLaunchKernelGGL((att_kernel<2, 1, true>), grid, block, 0, s, a);
-        else if (a.c.nb <= 4) hipLaunchKernelGGL((att_kernel<4, 1, true>), grid, block, 0, s, a);
-        else hipLaunchKernelGGL((att_kernel<8, 1, true>), grid, block, 0, s, a);
-        const int rc = launch_status();
-        if (rc != KORE_HIP_OK) return rc;
-    }
-    if (p.splits == 1) return KORE_HIP_OK;
-    for (a.tile0 = 0; a.tile0 < p.tiles; a.tile0 += band) {
-        const dim3 grid(std::min(band, p.tiles - a.tile0), (uint32_t)kv_heads);
-        hipLaunchKernelGGL(att_combine_kernel<16>, grid, dim3(kAttCombine), 0, s, a);
-        const int rc = launch_status();
-        if (rc != KORE_HIP_OK) return rc;
+    // A launch holds fewer than 2^32 threads: items in bands.
+    const uint32_t band = (uint32_t)std::max<uint64_t>(1, 0x400000u / kv_heads);
+    for (int join = 0; join < (p.target ? 2 : 1); ++join) {
+        for (a.item0 = 0; a.item0 < p.items; a.item0 += band) {
+            const uint32_t x = std::min(band, p.items - a.item0) * (uint32_t)kv_heads;
+            att_launch(a, p, join != 0, dim3(x), (hipStream_t)stream);
+            const int rc = launch_status();
+            if (rc != KORE_HIP_OK) return rc;
+        }
     }
     return KORE_HIP_OK;
 }

@@ -29,7 +29,7 @@ constexpr uint32_t kQkVecHeadDim = 512;  // 64 lanes a row
 constexpr int kQkBlock = 128;
 constexpr int kQkBwBlock = 256;
 constexpr uint32_t kQkBwTile = 8;       // tokens whose cos/sin lie in LDS
-constexpr uint32_t kQkBwParts = 2048;   // partial dw rows at most
+constexpr uint32_t kQkBwParts = 1024;   // partial dw rows at most
 
 struct QkArgs {
     const float* x[2];   // q, k
@@ -312,23 +312,37 @@ __global__ __launch_bounds__(kQkBwBlock) void qk_norm_rope_bwd_any_kernel(QkArgs
     }
 }
 
-// dw[t][d] = the partial rows' sum, in a fixed order: 16 row slots a column.
-constexpr int kQkRedCols = 16;
-__global__ __launch_bounds__(kQkBwBlock) void qk_norm_rope_dw_kernel(const float* part, uint32_t parts, uint32_t dim,
-                                                                     float* dqw, float* dkw) {
-    constexpr uint32_t kSlots = kQkBwBlock / kQkRedCols;
-    __shared__ float red[kSlots][kQkRedCols + 1];
-    const uint32_t col = blockIdx.x * kQkRedCols + threadIdx.x % kQkRedCols, slot = threadIdx.x / kQkRedCols;
+// dw[t][d] = the partial rows' sum, in a fixed order: 64 row slots a column, eight
+// rows of a slot in flight.
+constexpr int kQkRedCols = 16, kQkRedSlots = 64, kQkRedFlight = 8;
+__global__ __launch_bounds__(kQkRedCols* kQkRedSlots) void qk_norm_rope_dw_kernel(const float* part, uint32_t parts,
+                                                                                  uint32_t dim, float* dqw, float* dkw) {
+    __shared__ float red[kQkRedSlots][kQkRedCols + 1];
+    const uint32_t c = threadIdx.x % kQkRedCols, slot = threadIdx.x / kQkRedCols;
+    const uint32_t col = blockIdx.x * kQkRedCols + c;
     float s = 0.0f;
-    if (col < 2 * dim)
-        for (uint32_t p = slot; p < parts; p += kSlots) s += part[(uint64_t)p * 2 * dim + col];
-    red[slot][threadIdx.x % kQkRedCols] = s;
-    __syncthreads();
-    if (slot || col >= 2 * dim) return;
+    if (col < 2 * dim) {
+        for (uint32_t p = slot; p < parts; p += kQkRedSlots * kQkRedFlight) {
+            float v[kQkRedFlight];
 #pragma unroll
-    for (uint32_t v = 1; v < kSlots; ++v) s += red[v][threadIdx.x];
+            for (int i = 0; i < kQkRedFlight; ++i) {
+                const uint32_t at = p + i * kQkRedSlots;
+                v[i] = at < parts ? part[(uint64_t)at * 2 * dim + col] : 0.0f;
+            }
+#pragma unroll
+            for (int i = 0; i < kQkRedFlight; ++i) s += v[i];
+        }
+    }
+    red[slot][c] = s;
+    __syncthreads();
+#pragma unroll
+    for (int n = kQkRedSlots / 2; n >= 1; n /= 2) {
+        if (slot < (uint32_t)n) red[slot][c] += red[slot + n][c];
+        __syncthreads();
+    }
+    if (slot || col >= 2 * dim) return;
     float* o = col < dim ? dqw : dkw;
-    if (o) o[col < dim ? col : col - dim] = s;
+    if (o) o[col < dim ? col : col - dim] = red[0][c];
 }
 
 // Whether rows of `wa` floats every `sa` from a meet rows of `wb` every `sb`
@@ -348,7 +362,7 @@ struct QkPlan {
     uint32_t parts;  // workgroups, each a partial dw row
 };
 
-// Tiles of up to eight tokens once there are enough of them for 2048
+// Tiles of up to eight tokens once there are enough of them for 1024
 // workgroups, which then share the tiles.
 static QkPlan qk_plan(uint64_t tokens) {
     const uint32_t tile = (uint32_t)std::min<uint64_t>(kQkBwTile, std::max<uint64_t>(1, tokens / kQkBwParts));
@@ -545,8 +559,8 @@ extern "C" int kore_hip_qk_norm_rope_backward_f32(
         const int rc = launch_status();
         if (rc != KORE_HIP_OK) return rc;
     }
-    hipLaunchKernelGGL(qk_norm_rope_dw_kernel, dim3((2 * head_dim + kQkRedCols - 1) / kQkRedCols), dim3(kQkBwBlock), 0,
-                       s, workspace, a.tokens ? plan.parts : 0u, head_dim, q_heads ? grad_q_weight : nullptr,
+    hipLaunchKernelGGL(qk_norm_rope_dw_kernel, dim3((2 * head_dim + kQkRedCols - 1) / kQkRedCols),
+                       dim3(kQkRedCols * kQkRedSlots), 0, s, workspace, a.tokens ? plan.parts : 0u, head_dim, q_heads ? grad_q_weight : nullptr,
                        k_heads ? grad_k_weight : nullptr);
     return launch_status();
 }
