@@ -3,7 +3,7 @@
 //
 // One pass over the keys with the running maximum and sum of the softmax; no
 // scores in memory.  The rows of one key head are its query heads times the
-// sequence's new tokens: row r = token * group + head, 16 to a matrix tile.
+// sequence's new tokens: row r = token * group + head.
 //
 // Arithmetic.  A cached value is a code times a power of two, exact in bf16, and
 // gfx950 makes two of them with their scale in one instruction, so the matrix
@@ -17,17 +17,12 @@
 // E4M3 terms; but its sum keeps only some 2^-19 of the largest product, so blocks
 // of very different scales would cost accuracy that f32 has.)
 //
-// Layout of a step (32 tokens; n = lane % 16, g = lane / 16):
-//   S^T = K Q^T   a lane holds token n's dimensions of group g (K's codes as
-//                 they lie, 16 bytes at head_dim 128) and row n's same
-//                 dimensions: which eight of them meet in one product is free.
-//                 It gets tokens 4g .. 4g + 3 of row n.
-//   O^T = V^T P^T the operand P^T wants eight tokens of row n from lane group g:
-//                 the four it has of this 16-token tile and the four of the
-//                 next.  V's operand is taken in the same order of tokens, so P
-//                 moves between no lanes and through no memory.
-// All of a lane's values belong to row n: maximum, sum and rescaling are its
-// own, but for a maximum over the four lane groups.
+// Both products are taken transposed, S^T = K Q^T and O^T = V^T P^T, so that a
+// lane's scores, probabilities and outputs all belong to one row, its column:
+// maximum, sum and rescaling are its own, but for a maximum over the four lane
+// groups.  The operand P^T wants eight tokens of a row from each lane group; V's
+// operand is taken for those eight that the lane has from S^T, so P moves between
+// no lanes and through no memory.
 //
 // A masked token's score is -inf whatever its codes say.  Its V is finite (the
 // scale of a token past the cache's length counts as 1); where V of a token
@@ -46,11 +41,11 @@ typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
 constexpr int kAttBlock = 256;
 constexpr int kAttWaves = kAttBlock / kWave;
-constexpr uint32_t kAttStep = 32;      // tokens of a step
-constexpr uint32_t kAttMinChunk = 8;   // steps of a split, at least
-constexpr uint32_t kAttMaxSteps = 1u << 27;  // more than 2^31 keys have
-constexpr int kAttTerms = 3;           // bf16 terms of a query value
-constexpr uint32_t kAttJoin = 512;  // threads of the joining kernel
+constexpr uint32_t kAttStep = 32;             // tokens of a step
+constexpr uint32_t kAttMinChunk = 8;          // steps of a share, at least
+constexpr uint32_t kAttMaxSteps = 1u << 27;   // more than 2^31 keys have
+constexpr int kAttTerms = 3;                  // bf16 terms of a query value
+constexpr uint32_t kAttJoin = 512;            // threads of the joining kernel
 constexpr uint32_t kAttMaxSplits = 1024;
 
 struct AttArgs {
@@ -187,6 +182,21 @@ template <int kSel>
 __device__ __forceinline__ uint32_t cvt2(uint32_t codes, float scale) {
     return __builtin_bit_cast(uint32_t, (bf16x2)__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, kSel));
 }
+// Eight codes.
+__device__ __forceinline__ u32x4 cvt8(uint32_t codes, float scale) {
+    return {cvt2<0>(codes, scale), cvt2<1>(codes, scale), cvt2<2>(codes, scale), cvt2<3>(codes, scale)};
+}
+// Pair `sel` (a constant) of eight codes.
+__device__ __forceinline__ uint32_t cvt_pair(uint32_t codes, float scale, int sel) {
+    return sel == 0   ? cvt2<0>(codes, scale)
+           : sel == 1 ? cvt2<1>(codes, scale)
+           : sel == 2 ? cvt2<2>(codes, scale)
+                      : cvt2<3>(codes, scale);
+}
+// The scale in byte i of four.
+__device__ __forceinline__ float byte_scale(uint32_t bytes, int i) {
+    return __uint_as_float((bytes >> 8 * i & 0xffu) << 23);
+}
 
 __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0,
@@ -207,16 +217,35 @@ __device__ __forceinline__ const float* att_query(const AttArgs& a, const AttIte
     return a.q + (uint64_t)(t.q0 + r / a.group) * a.q_stride + (uint64_t)(head * a.group + r % a.group) * a.dim;
 }
 
-// What a lane loads of one 16-token tile.
-template <int NB>
-struct AttKV {
-    static constexpr int kC = NB < 4 ? 1 : NB / 4;  // 16-byte pieces
-    uint32_t k[NB];   // token n's codes of group g, eight dimensions a dword
-    u32x4 v[kC];      // four tokens of chunk n (or n / 2, or 2n and 2n + 1)
-    uint32_t ks[kC];  // K's scale bytes
-    uint32_t vs;      // V's scale bytes of tokens 4g .. 4g + 3
-    uint32_t valid;   // tokens of the tile that exist
-};
+// Eight values of a query row from dimension d on, scaled, as its three terms of
+// eight bf16: the top 16 bits, then those of what they leave.
+__device__ __forceinline__ void query_terms(const AttArgs& a, const float* q, uint32_t d, bool live,
+                                            u32x4 (&term)[kAttTerms]) {
+    float x[8];
+    if (live && d + 8 <= a.dim) {
+        const f32x4 u = (f32x4)*reinterpret_cast<const f32x4_a4*>(q + d);
+        const f32x4 v = (f32x4)*reinterpret_cast<const f32x4_a4*>(q + d + 4);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            x[i] = u[i];
+            x[4 + i] = v[i];
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = live && d + i < a.dim ? q[d + i] : 0.0f;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        float u = x[2 * i] * a.scale_log2, v = x[2 * i + 1] * a.scale_log2;
+#pragma unroll
+        for (int k = 0; k < kAttTerms; ++k) {
+            const uint32_t ub = __float_as_uint(u), vb = __float_as_uint(v);
+            term[k][i] = perm(vb, ub, 0x07060302u);
+            u -= __uint_as_float(ub & 0xffff0000u);
+            v -= __uint_as_float(vb & 0xffff0000u);
+        }
+    }
+}
 
 // A value that the compiler takes as new, so that 32-bit offsets stay 32 bits wide
 // beside their use (a load from a scalar base) and no 64-bit sums are kept.
@@ -231,30 +260,153 @@ __device__ __forceinline__ float add_ror(float v) {
     return v + __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0x120 + N, 0xf, 0xf, true));
 }
 
+// Where a step's tiles of 16 tokens lie: the page table through scalar loads,
+// which have a counter of their own.  A tile past the end, or of a page that does
+// not exist, is one of page 0 with no tokens: loads have no conditions on their
+// way, so that a step's can be waited for while the next one's are in flight.
+struct AttPages {
+    typedef const __attribute__((address_space(4))) uint32_t* ScalarPtr;
+    ScalarPtr table;
+    const uint8_t* cache;
+    uint32_t last, shift, kv_len, num_pages, page;
+    uint64_t page_bytes;
+
+    __device__ AttPages(const AttArgs& a, const AttItem& t, uint32_t head)
+        : table((ScalarPtr)(uintptr_t)(a.table + (uint64_t)t.seq * a.max_pages)),
+          cache(a.cache + (uint64_t)head * a.c.head_bytes),
+          last(t.kv_len ? (t.kv_len - 1) >> a.c.shift : 0),
+          shift(a.c.shift),
+          kv_len(t.kv_len),
+          num_pages(a.c.num_pages),
+          page(a.c.page),
+          page_bytes(a.c.page_bytes) {}
+
+    __device__ uint32_t id(uint32_t tt) const { return table[min(tt * 16 >> shift, last)]; }
+    // Tile tt of page `id`: its piece of the page, its tokens, the first's place.
+    __device__ const uint8_t* at(uint32_t tt, uint32_t id, uint32_t* valid, uint32_t* t0) const {
+        *valid = min(kv_len - min(kv_len, tt * 16), 16u);
+        if (id >= num_pages) id = 0, *valid = 0;
+        *t0 = (tt * 16) & (page - 1);
+        return cache + (uint64_t)id * page_bytes;
+    }
+};
+
+// V's four scale bytes of tokens first .. first + 3 of a tile that rows may not see
+// all of: 1 for tokens that do not exist, and for NaN, which is reported.
+__device__ __forceinline__ uint32_t finite_scales(uint32_t bytes, uint32_t first, uint32_t valid, bool* nan) {
+    uint32_t out = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        uint32_t b = bytes >> 8 * i & 0xffu;
+        if (first + i >= valid) b = 127;
+        if (b == kQ4NanScale) *nan = true, b = 127;
+        out |= b << 8 * i;
+    }
+    return out;
+}
+
+// Blocks of V (bits) in which a token of tile tt that the lane's row sees is NaN.
+// For steps that some rows see a part of: what their product takes instead is 1.
+__device__ __forceinline__ uint32_t nan_blocks(const AttArgs& a, const AttPages& pages, uint32_t tt, uint32_t id,
+                                            uint32_t limit) {
+    uint32_t valid, t0, bits = 0;
+    const uint8_t* base = pages.at(tt, id, &valid, &t0);
+    for (uint32_t b = 0; b < a.c.nb; ++b)
+        for (uint32_t i = 0; i < valid; ++i)
+            if (base[q4_v_scale(a.c, t0 + i, b)] == kQ4NanScale && tt * 16 + i < limit) bits |= 1u << b;
+    return bits;
+}
+
+// A row's running maximum, as what its probabilities are relative to.  It rises
+// only when a score passes it by more than 2^8, so that sums and outputs are seldom
+// rescaled; probabilities of up to 2^8 change no rounding.
+struct AttMax {
+    static constexpr float kSlack = 8.0f;
+    float base = 0.0f, limit = -__builtin_inff();  // limit: -inf before the first score, then base + kSlack
+
+    __device__ float value() const { return limit == -__builtin_inff() ? limit : base; }
+    // Scores of at most mx: what sums and outputs so far have to be multiplied by.
+    __device__ float rise(float mx) {
+        if (!(mx > limit)) return 1.0f;
+        // before the first score there is nothing (or NaN) to rescale
+        const float f = limit == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(base - mx);
+        base = mx;
+        limit = mx + kSlack;
+        return f;
+    }
+};
+
+// `kCount` values from dimension d on of the sequence's row rr, not yet divided by
+// its sum l: to the output, or with its maximum m to the share's part.
+template <uint32_t kRows, int kCount>
+__device__ __forceinline__ void att_store(const AttArgs& a, const AttItem& t, uint32_t item, uint32_t head, uint32_t rr,
+                                          float m, float l, uint32_t d, const float (&v)[kCount]) {
+    if (t.splits > 1) {
+        const uint32_t dp = 32 * a.c.nb;
+        const uint64_t at = ((uint64_t)item * a.c.kv_heads + head) * kRows + (rr - t.first);
+        if (d == 0) *reinterpret_cast<float2*>(a.part + at * 2) = make_float2(m, l);
+        float* p = a.part + (uint64_t)a.items * a.c.kv_heads * kRows * 2 + at * dp + d;
+#pragma unroll
+        for (int i = 0; i < kCount; i += 4)
+            if (d + i < dp) *reinterpret_cast<f32x4*>(p + i) = {v[i], v[i + 1], v[i + 2], v[i + 3]};
+        return;
+    }
+    const float f = l == 0.0f ? 0.0f : 1.0f / l;
+    float* p = a.out + ((uint64_t)(t.q0 + rr / a.group) * a.q_heads + head * a.group + rr % a.group) * a.dim + d;
+#pragma unroll
+    for (int i = 0; i < kCount; i += 4) {
+        float u[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) u[k] = l == 0.0f ? 0.0f : v[i + k] * f;
+        if (d + i + 4 <= a.dim) {
+            *reinterpret_cast<f32x4_a4*>(p + i) = {u[0], u[1], u[2], u[3]};
+        } else {
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                if (d + i + k < a.dim) p[i + k] = u[k];
+        }
+    }
+}
+
+// What a lane (n = lane % 16, g = lane / 16) loads of one 16-token tile.
+template <int NB>
+struct AttKV {
+    static constexpr int kC = NB < 4 ? 1 : NB / 4;  // 16-byte pieces
+    uint32_t k[NB];   // token n's codes of group g, eight dimensions a dword
+    u32x4 v[kC];      // four tokens of chunk n (or n / 2, or 2n and 2n + 1)
+    uint32_t ks[kC];  // K's scale bytes
+    uint32_t vs;      // V's scale bytes of tokens 4g .. 4g + 3
+    uint32_t valid;   // tokens of the tile that exist
+};
+
 // NB: blocks of 32 dimensions that the tiles hold (2, 4 or 8), nb <= NB of them
-// in use.  kSlot: query rows of a matrix tile's 16 columns.  16: a product for
-// each of q's three terms and each of p's two.  With 8 or 4 rows (a decode step's
-// query heads) the terms lie side by side in the columns instead, column = slot *
-// kSlot + row: one product takes two or all three of q's terms and both of p's,
-// and the slots' scores are added across lanes.
-// R: 16-row tiles of a wave.  An item's rows are kSlot, or 64 R: its waves deal
-// out the rows, and where there are too few rows for four waves, the tokens,
-// whose parts they join at the end.
+// in use.  kSlot: rows of a matrix tile's 16 columns.  16: a product for each of
+// q's three terms and each of p's two.  With 8 or 4 rows (a decode step's query
+// heads) the terms lie side by side in the columns instead, column = slot * kSlot +
+// row: one product takes two or all three of q's terms and both of p's, and the
+// slots' scores are added across lanes.
+// R: 16-row tiles of a wave.  An item's rows are kSlot, or with R = 2 four waves'
+// 128: the waves deal out the rows, and where there are too few rows for four
+// waves, the tokens, whose parts they join at the end.
 template <int NB, int R, int kSlot>
 struct AttShape {
     static constexpr uint32_t kWaveRows = kSlot < 16 ? kSlot : 16 * R;
     static constexpr uint32_t kRows = kSlot < 16 ? kSlot : 16 * R * kAttWaves;
-    static constexpr int kSide = 16 / kSlot;                      // terms side by side
-    static constexpr int kQ = (kAttTerms + kSide - 1) / kSide;    // products for a score
-    static constexpr int kP = kSlot == 16 ? 2 : 1;                // products for an output
+    static constexpr int kSide = 16 / kSlot;                       // terms side by side
+    static constexpr int kQ = (kAttTerms + kSide - 1) / kSide;     // products for a score
+    static constexpr int kP = kSlot == 16 ? 2 : 1;                 // products for an output
 };
 
+// A step, v_mfma_f32_16x16x32_bf16: for S^T a lane holds token n's dimensions of
+// group g (K's codes as they lie, 16 bytes at head_dim 128; which eight of them
+// meet in one product is free, q's operand is taken alike) and gets tokens 4g ..
+// 4g + 3 of row n, for two tiles; for O^T those are its eight tokens.
 template <int NB, int R, int kSlot, int kPerSimd>
 __global__ __launch_bounds__(kAttBlock) __attribute__((amdgpu_waves_per_eu(kPerSimd, kPerSimd)))
 void att_kernel(AttArgs a) {
     using Shape = AttShape<NB, R, kSlot>;
     constexpr uint32_t kRows = Shape::kRows, kWaveRows = Shape::kWaveRows;
-    constexpr int kQ = Shape::kQ, kP = Shape::kP, kC = AttKV<NB>::kC;
+    constexpr int kQ = Shape::kQ, kP = Shape::kP, kC = AttKV<NB>::kC, kSide = Shape::kSide;
     constexpr int kJ = 2 * NB;  // dimensions of a lane's part of a row, and O tiles
     const uint32_t lane = threadIdx.x % kWave, n = lane % 16, g = lane / 16;
     const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x / kWave));
@@ -264,65 +416,40 @@ void att_kernel(AttArgs a) {
     const AttItem t = att_item<kRows>(a, item);
     if (!t.ok) return;
     const uint32_t nb = a.c.nb;
+    // The item's share of its steps: [lo, hi).
+    const uint32_t steps = att_steps(att_limit(a, t, min(t.first + kRows, t.rows) - 1));
+    const uint32_t lo = t.splits > 1 ? t.split * t.chunk : 0, hi = t.splits > 1 ? min(lo + t.chunk, steps) : steps;
+    if (t.splits > 1 && lo >= hi) return;  // the joining kernel knows
     // The waves' rows: one, two or four groups of them; the waves of a group share
     // its tokens.
     const uint32_t left = min(t.rows - t.first, kRows);
     const uint32_t groups = left <= kWaveRows ? 1 : left <= 2 * kWaveRows ? 2 : 4;
-    const uint32_t share_of = kAttWaves / groups, part = wave / groups;
+    const uint32_t stride = kAttWaves / groups;
     const uint32_t r0 = t.first + (wave % groups) * kWaveRows;  // the wave's first row
     const uint32_t r1 = min(r0 + kWaveRows, t.rows);            // its end; r0 or less: no rows
-    const uint32_t last_row = min(t.first + kRows, t.rows) - 1;
-
-    // Tokens of this split, then of this wave.
-    const uint32_t steps = att_steps(att_limit(a, t, last_row));
-    const uint32_t lo = t.splits > 1 ? t.split * t.chunk : 0, hi = t.splits > 1 ? min(lo + t.chunk, steps) : steps;
-    if (t.splits > 1 && lo >= hi) return;  // the joining kernel knows
     const uint32_t min_limit = att_limit(a, t, min(r0, t.rows - 1));
     const uint32_t end = r0 < r1 ? min(hi, att_steps(att_limit(a, t, r1 - 1))) : 0;
 
+    const uint32_t slot = n / kSlot;
     uint32_t limit[R];
     u32x4 qf[R][kQ][NB];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-        const uint32_t row = r0 + 16 * r + n % kSlot, slot = n / kSlot;
+        const uint32_t row = r0 + 16 * r + n % kSlot;
         const bool live = row < r1;
         limit[r] = live ? att_limit(a, t, row) : 0;
         const float* qp = att_query(a, t, head, live ? row : 0);
 #pragma unroll
         for (int j = 0; j < NB; ++j) {
-            const uint32_t d0 = g * 8 * NB + 8 * j;
-            float x[8];
-            if (live && d0 + 8 <= a.dim) {
-                const f32x4 u = (f32x4)*reinterpret_cast<const f32x4_a4*>(qp + d0);
-                const f32x4 v = (f32x4)*reinterpret_cast<const f32x4_a4*>(qp + d0 + 4);
+            u32x4 term[kAttTerms];
+            query_terms(a, qp, g * 8 * NB + 8 * j, live, term);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    x[i] = u[i];
-                    x[4 + i] = v[i];
-                }
-            } else {
+            for (int k = 0; k < kQ; ++k) {
+                u32x4 w = {0, 0, 0, 0};
 #pragma unroll
-                for (int i = 0; i < 8; ++i) x[i] = live && d0 + i < a.dim ? qp[d0 + i] : 0.0f;
-            }
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                float u = x[2 * i] * a.scale_log2, v = x[2 * i + 1] * a.scale_log2;
-                uint32_t term[kAttTerms];
-#pragma unroll
-                for (int k = 0; k < kAttTerms; ++k) {  // the top 16 bits, then what they leave
-                    const uint32_t ub = __float_as_uint(u), vb = __float_as_uint(v);
-                    term[k] = perm(vb, ub, 0x07060302u);
-                    u -= __uint_as_float(ub & 0xffff0000u);
-                    v -= __uint_as_float(vb & 0xffff0000u);
-                }
-#pragma unroll
-                for (int k = 0; k < kQ; ++k) {
-                    uint32_t w = 0;
-#pragma unroll
-                    for (int at = 0; at < Shape::kSide; ++at)
-                        if (k * Shape::kSide + at < kAttTerms && slot == (uint32_t)at) w = term[k * Shape::kSide + at];
-                    qf[r][k][j][i] = w;
-                }
+                for (int at = 0; at < kSide; ++at)
+                    if (k * kSide + at < kAttTerms && slot == (uint32_t)at) w = term[k * kSide + at];
+                qf[r][k][j] = w;
             }
         }
     }
@@ -330,24 +457,20 @@ void att_kernel(AttArgs a) {
     const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
     const float ninf = -__builtin_inff();
     f32x4 o[R][kJ];
-    float m[R], l[R];
+    AttMax top[R];
+    float l[R];
+    uint32_t poison[R];  // blocks of V in which the row sees NaN that others do not
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-        m[r] = ninf;
         l[r] = 0.0f;
+        poison[r] = 0;
 #pragma unroll
         for (int j = 0; j < kJ; ++j) o[r][j] = zero;
     }
 
-    // Loads have no conditions on their way, so that a step's can be waited for
-    // while the next one's are in flight: a tile past the end is one of page 0 with
-    // no tokens, blocks past nb are read from the last one (q is zero there, and
-    // what they add to the output is not stored).
-    typedef const __attribute__((address_space(4))) uint32_t* ScalarPtr;
-    const ScalarPtr table = (ScalarPtr)(uintptr_t)(a.table + (uint64_t)t.seq * a.max_pages);
-    const uint32_t last_page = t.kv_len ? (t.kv_len - 1) >> a.c.shift : 0;
-    auto page_of = [&](uint32_t tt) { return table[min(tt * 16 >> a.c.shift, last_page)]; };
-    const uint32_t stride = share_of;
+    // Blocks past nb are read from the last one: q is zero there, and what they add
+    // to the output is not stored.
+    const AttPages pages(a, t, head);
     uint32_t koff[kC], ksoff[kC], voff[kC], vsoff = 0;
 #pragma unroll
     for (int c = 0; c < kC; ++c) {
@@ -359,10 +482,8 @@ void att_kernel(AttArgs a) {
         if (c == 0) vsoff = np * 33 + chunk / 4 * 16 + 4 * g;
     }
     auto load = [&](uint32_t tt, uint32_t page, AttKV<NB>& x) {
-        x.valid = min(t.kv_len - min(t.kv_len, tt * 16), 16u);
-        if (page >= a.c.num_pages) page = 0, x.valid = 0;  // a page that does not exist has no tokens
-        const uint32_t t0 = (tt * 16) & (a.c.page - 1);
-        const uint8_t* base = a.cache + (uint64_t)page * a.c.page_bytes + (uint64_t)head * a.c.head_bytes;
+        uint32_t t0;
+        const uint8_t* base = pages.at(tt, page, &x.valid, &t0);
         const uint8_t* codes = base + t0 * nb * 16;
         const uint8_t* scales = base + t0 * nb;
 #pragma unroll
@@ -382,8 +503,8 @@ void att_kernel(AttArgs a) {
         x.vs = *reinterpret_cast<const uint32_t*>(scales + opaque(vsoff));
     };
 
-    auto work = [&](uint32_t step, AttKV<NB> (&cur)[2], uint32_t page0, uint32_t page1) {
-        // Scores: tokens 4g + i of both tiles, in powers of two.
+    auto work = [&](uint32_t step, AttKV<NB> (&cur)[2], const uint32_t (&page)[2]) {
+        // Scores, in powers of two: tokens 4g + i of both tiles.
         f32x4 s[R][2];
 #pragma unroll
         for (int r = 0; r < R; ++r) s[r][0] = s[r][1] = zero;
@@ -391,9 +512,7 @@ void att_kernel(AttArgs a) {
         for (int j = 0; j < NB; ++j)
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
-                const float sc = __uint_as_float(cur[x].ks[j / 4] << 23);
-                const uint32_t code = cur[x].k[j];
-                const u32x4 kf = {cvt2<0>(code, sc), cvt2<1>(code, sc), cvt2<2>(code, sc), cvt2<3>(code, sc)};
+                const u32x4 kf = cvt8(cur[x].k[j], byte_scale(cur[x].ks[j / 4], 0));
 #pragma unroll
                 for (int k = kQ - 1; k >= 0; --k)
 #pragma unroll
@@ -415,21 +534,14 @@ void att_kernel(AttArgs a) {
         if (!whole) {
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
-                const uint32_t have_x = at + 16 * x + cur[x].valid;  // the tile's tokens end here
 #pragma unroll
-                for (int r = 0; r < R; ++r)
+                for (int r = 0; r < R; ++r) {
+                    const uint32_t have = min(limit[r], at + 16 * x + cur[x].valid);
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
-                        if (at + 16 * x + 4 * g + i >= min(limit[r], have_x)) s[r][x][i] = ninf;
-                uint32_t vs = 0;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    uint32_t b = cur[x].vs >> 8 * i & 0xffu;
-                    if (4 * g + i >= cur[x].valid) b = 127;
-                    if (b == kQ4NanScale) nan_v = true, b = 127;
-                    vs |= b << 8 * i;
+                        if (at + 16 * x + 4 * g + i >= have) s[r][x][i] = ninf;
                 }
-                cur[x].vs = vs;
+                cur[x].vs = finite_scales(cur[x].vs, 4 * g, cur[x].valid, &nan_v);
             }
         }
         // Running maximum, probabilities and their sum; bf16 terms.
@@ -438,31 +550,28 @@ void att_kernel(AttArgs a) {
         for (int r = 0; r < R; ++r) {
             float mx = fmaxf(fmaxf(fmaxf(s[r][0][0], s[r][0][1]), fmaxf(s[r][0][2], s[r][0][3])),
                              fmaxf(fmaxf(s[r][1][0], s[r][1][1]), fmaxf(s[r][1][2], s[r][1][3])));
-            if (__any(mx > m[r])) {
+            if (__any(mx > top[r].limit)) {
                 mx = fmaxf(mx, __shfl_xor(mx, 16, kWave));
                 mx = fmaxf(mx, __shfl_xor(mx, 32, kWave));
-                const float mn = fmaxf(m[r], mx);
-                const float f = mn > m[r] ? __builtin_amdgcn_exp2f(m[r] - mn) : 1.0f;
-                m[r] = mn;
+                const float f = top[r].rise(mx);
                 l[r] *= f;
 #pragma unroll
                 for (int j = 0; j < kJ; ++j) o[r][j] *= f;
             }
-            const float base = m[r] == ninf ? 0.0f : m[r];
 #pragma unroll
             for (int x = 0; x < 2; ++x)
 #pragma unroll
                 for (int i = 0; i < 4; i += 2) {
-                    float p0 = __builtin_amdgcn_exp2f(s[r][x][i] - base);
-                    float p1 = __builtin_amdgcn_exp2f(s[r][x][i + 1] - base);
+                    const float p0 = __builtin_amdgcn_exp2f(s[r][x][i] - top[r].base);
+                    const float p1 = __builtin_amdgcn_exp2f(s[r][x][i + 1] - top[r].base);
                     l[r] += p0 + p1;
                     float e0, e1, u0, u1;
-                    const uint32_t top = pack_bf16(p0, p1, &e0, &e1);
+                    const uint32_t first = pack_bf16(p0, p1, &e0, &e1);
                     if constexpr (kSlot == 16) {
-                        pf[r][0][2 * x + i / 2] = top;
+                        pf[r][0][2 * x + i / 2] = first;
                         pf[r][1][2 * x + i / 2] = pack_bf16(e0, e1, &u0, &u1);
                     } else {  // slot 0 holds the first term, slot 1 the second; the others are not read
-                        pf[r][0][2 * x + i / 2] = n < kSlot ? top : pack_bf16(e0, e1, &u0, &u1);
+                        pf[r][0][2 * x + i / 2] = slot ? pack_bf16(e0, e1, &u0, &u1) : first;
                     }
                 }
         }
@@ -470,7 +579,7 @@ void att_kernel(AttArgs a) {
         // eight tokens of one dimension.
         float vsc[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) vsc[i] = __uint_as_float((cur[i >> 2].vs >> 8 * (i & 3) & 0xffu) << 23);
+        for (int i = 0; i < 8; ++i) vsc[i] = byte_scale(cur[i >> 2].vs, i & 3);
 #pragma unroll
         for (int p = 0; p < NB; ++p) {  // pair of dimensions 2p, 2p + 1
             uint32_t v[8];
@@ -478,10 +587,7 @@ void att_kernel(AttArgs a) {
             for (int i = 0; i < 8; ++i) {
                 uint32_t code = cur[i >> 2].v[NB == 8 ? p >> 2 : 0][i & 3];
                 if (NB == 2) code >>= (n & 1) * 16;  // the lane's four dimensions of the chunk
-                v[i] = (p & 3) == 0   ? cvt2<0>(code, vsc[i])
-                       : (p & 3) == 1 ? cvt2<1>(code, vsc[i])
-                       : (p & 3) == 2 ? cvt2<2>(code, vsc[i])
-                                      : cvt2<3>(code, vsc[i]);
+                v[i] = cvt_pair(code, vsc[i], p & 3);
             }
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
@@ -494,99 +600,57 @@ void att_kernel(AttArgs a) {
                     for (int r = 0; r < R; ++r) o[r][2 * p + h] = mfma(vf, pf[r][k], o[r][2 * p + h]);
             }
         }
-        // A NaN block of a token that some rows do not see: its 32 dimensions of
-        // the rows that do.
         if (!whole && __any(nan_v)) {
-            for (uint32_t x = 0; x < 2; ++x) {
-                const uint32_t page = x ? page1 : page0, t0 = (at + 16 * x) & (a.c.page - 1);
-                const uint32_t valid = x ? cur[1].valid : cur[0].valid;
-                const uint8_t* base = a.cache + (uint64_t)page * a.c.page_bytes + (uint64_t)head * a.c.head_bytes;
-                for (uint32_t b = 0; b < nb; ++b)
-                    for (uint32_t i = 0; i < valid; ++i)
-                        if (base[q4_v_scale(a.c, t0 + i, b)] == kQ4NanScale)
 #pragma unroll
-                            for (int r = 0; r < R; ++r)
-                                if (at + 16 * x + i < limit[r])
+            for (int x = 0; x < 2; ++x)
 #pragma unroll
-                                    for (int k = 0; k < 4; ++k)
-                                        if ((NB * (4 * g + k)) / 16 == b)
-#pragma unroll
-                                            for (int j = 0; j < kJ; ++j) o[r][j][k] = __uint_as_float(0x7fc00000u);
-            }
+                for (int r = 0; r < R; ++r) poison[r] |= nan_blocks(a, pages, 2 * step + x, page[x], limit[r]);
         }
     };
 
     // Two steps in turn: one's loads are in flight while the other is worked on,
     // the pages of the one after that on their way.
-    uint32_t step = lo + part;
+    uint32_t step = lo + wave / groups;
     if (step < end) {
         AttKV<NB> kv[2][2];
-        uint32_t pg[2][2], ahead[2];
+        uint32_t page[2][2], ahead[2];
         auto fetch = [&](uint32_t st, int to) {
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
-                pg[to][x] = ahead[x];
+                page[to][x] = ahead[x];
                 load(2 * st + x, ahead[x], kv[to][x]);
             }
 #pragma unroll
-            for (int x = 0; x < 2; ++x) ahead[x] = page_of(2 * (st + stride) + x);
+            for (int x = 0; x < 2; ++x) ahead[x] = pages.id(2 * (st + stride) + x);
         };
-        ahead[0] = page_of(2 * step);
-        ahead[1] = page_of(2 * step + 1);
+        ahead[0] = pages.id(2 * step);
+        ahead[1] = pages.id(2 * step + 1);
         fetch(step, 0);
         for (;;) {
             fetch(step + stride, 1);
-            work(step, kv[0], pg[0][0], pg[0][1]);
+            work(step, kv[0], page[0]);
             step += stride;
             if (step >= end) break;
             fetch(step + stride, 0);
-            work(step, kv[1], pg[1][0], pg[1][1]);
+            work(step, kv[1], page[1]);
             step += stride;
             if (step >= end) break;
         }
     }
 
+    // Lane (n, g) has dimensions kJ (4g + i) + j of row n in o[.][j][i].
 #pragma unroll
     for (int r = 0; r < R; ++r) {
         l[r] += __shfl_xor(l[r], 16, kWave);
         l[r] += __shfl_xor(l[r], 32, kWave);
-    }
-    // Lane (n, g) has dimensions kJ (4g + i) + j of row n in o[.][j][i].
-    const uint64_t part0 = ((uint64_t)item * a.c.kv_heads + head) * kRows;
-    const uint32_t dp = 32 * nb;
-    float* const pm = a.part;  // [rows][2] of all, then [rows][dp] of all
-    float* const po = a.part + (uint64_t)a.items * a.c.kv_heads * kRows * 2;
-    // `count` values from dimension d of the sequence's row rr, not yet divided.
-    auto store_row = [&](uint32_t rr, float mm, float ll, uint32_t d, const float* v, auto count) {
-        constexpr int kCount = decltype(count)::value;
-        if (t.splits > 1) {
-            const uint64_t at = part0 + (rr - t.first);
-            if (d == 0) {
-                pm[at * 2] = mm;
-                pm[at * 2 + 1] = ll;
-            }
-            float* p = po + at * dp + d;
+        if (poison[r]) {
 #pragma unroll
-            for (int i = 0; i < kCount; i += 4)
-                if (d + i < dp) *reinterpret_cast<f32x4*>(p + i) = {v[i], v[i + 1], v[i + 2], v[i + 3]};
-        } else {
-            const float f = ll == 0.0f ? 0.0f : 1.0f / ll;
-            float* p = a.out + ((uint64_t)(t.q0 + rr / a.group) * a.q_heads + head * a.group + rr % a.group) * a.dim + d;
+            for (int i = 0; i < 4; ++i)
+                if (poison[r] >> NB * (4 * g + i) / 16 & 1)
 #pragma unroll
-            for (int i = 0; i < kCount; i += 4) {
-                float u[4];
-#pragma unroll
-                for (int k = 0; k < 4; ++k) u[k] = ll == 0.0f ? 0.0f : v[i + k] * f;
-                if (d + i + 4 <= a.dim) {
-                    *reinterpret_cast<f32x4_a4*>(p + i) = {u[0], u[1], u[2], u[3]};
-                } else {
-#pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                        if (d + i + k < a.dim) p[i + k] = u[k];
-                }
-            }
+                    for (int j = 0; j < kJ; ++j) o[r][j][i] = __uint_as_float(0x7fc00000u);
         }
-    };
+    }
     if (groups == kAttWaves) {
         if constexpr (kSlot == 16) {
 #pragma unroll
@@ -598,7 +662,7 @@ void att_kernel(AttArgs a) {
                     float v[kJ];
 #pragma unroll
                     for (int j = 0; j < kJ; ++j) v[j] = o[r][j][i];
-                    store_row(row, m[r], l[r], kJ * (4 * g + i), v, std::integral_constant<int, kJ>());
+                    att_store<kRows>(a, t, item, head, row, top[r].value(), l[r], kJ * (4 * g + i), v);
                 }
             }
         }
@@ -606,14 +670,13 @@ void att_kernel(AttArgs a) {
     }
     // Join the waves of a group: to the common maximum, then add (and the second
     // term's column to the first's).
-    constexpr int kPitch = 16 * kJ + 4;
     __shared__ float sm[kAttWaves][16], sl[kAttWaves][16];
-    __shared__ __attribute__((aligned(16))) float so[kAttWaves][16][kPitch];
+    __shared__ __attribute__((aligned(16))) float so[kAttWaves][16][16 * kJ + 4];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
         __syncthreads();
         if (g == 0) {
-            sm[wave][n] = m[r];
+            sm[wave][n] = top[r].value();
             sl[wave][n] = l[r];
         }
 #pragma unroll
@@ -629,9 +692,8 @@ void att_kernel(AttArgs a) {
             const uint32_t d = i % kQuads * 4, row = i / kQuads % kTall, gr = i / kQuads / kTall;
             const uint32_t rr = t.first + gr * kWaveRows + 16 * r + row;
             if (rr >= t.rows) continue;
-            float mm = ninf, ll = 0.0f;
+            float mm = ninf, ll = 0.0f, v[4] = {0.f, 0.f, 0.f, 0.f};
             for (uint32_t w = gr; w < kAttWaves; w += groups) mm = fmaxf(mm, sm[w][row]);
-            float v[4] = {0.f, 0.f, 0.f, 0.f};
             for (uint32_t w = gr; w < kAttWaves; w += groups) {
                 // a wave that saw nothing holds zeros (or NaN, which stays)
                 const float f = sm[w][row] == ninf ? 1.0f : __builtin_amdgcn_exp2f(sm[w][row] - mm);
@@ -641,7 +703,7 @@ void att_kernel(AttArgs a) {
 #pragma unroll
                 for (int k = 0; k < 4; ++k) v[k] += u[k] * f;
             }
-            store_row(rr, mm, ll, d, v, std::integral_constant<int, 4>());
+            att_store<kRows>(a, t, item, head, rr, mm, ll, d, v);
         }
     }
 }
@@ -703,11 +765,10 @@ __global__ __launch_bounds__(kAttJoin) void att_join_kernel(AttArgs a) {
     }
 }
 
-// Rows of an item: a decode step's query heads in a few columns, or rows for four
-// waves.
+// Rows of an item: a decode step's query heads in a few columns, or 32 for each of
+// four waves.
 struct AttPlan {
-    int slot, r;    // kSlot, R
-    uint32_t rows;  // kRows
+    uint32_t rows;  // kRows: 4, 8 (kSlot), 64 or 128 (kSlot 16)
     uint32_t items, target;
     uint64_t bytes;  // workspace
 };
@@ -715,16 +776,14 @@ struct AttPlan {
 static int att_plan(uint64_t num_seqs, uint64_t tokens, uint64_t q_heads, uint64_t kv_heads, uint64_t page_size,
                     uint64_t max_pages, uint32_t nb, AttPlan* p) {
     const uint64_t group = q_heads / kv_heads, rows = tokens * group;
-    p->slot = rows <= 4 * num_seqs ? 4 : rows <= 8 * num_seqs ? 8 : 16;
-    p->r = p->slot < 16 || nb > 4 ? 1 : 2;
-    p->rows = p->slot < 16 ? p->slot : 64u * p->r;
+    p->rows = rows <= 4 * num_seqs ? 4 : rows <= 8 * num_seqs ? 8 : rows <= 16 * num_seqs || nb > 4 ? 64 : 128;
     const uint64_t tiles = rows / p->rows + num_seqs;
     if (tiles > 0x3fffffull) return KORE_HIP_ERR_OVERFLOW;
     // Workgroups that the keys are cut for: what the chip holds at once.
-    const uint64_t want = p->slot == 4 && nb <= 4 ? 768 : 512;
+    const uint64_t want = p->rows == 4 && nb <= 4 ? 768 : 512;
     const uint64_t busy = std::max(std::min(num_seqs, tokens), rows / p->rows) * kv_heads;
     const uint64_t shares = max_pages * page_size / (kAttMinChunk * kAttStep);  // of the longest sequence
-    const bool cut = busy < (p->slot < 16 ? 2 * want : want / 2) && shares > 1;
+    const bool cut = busy < (rows <= 16 * num_seqs ? 2 * want : want / 2) && shares > 1;
     p->target = cut ? (uint32_t)std::min<uint64_t>({(want + kv_heads - 1) / kv_heads, tiles * shares, kAttMaxSplits}) : 0;
     p->items = std::max((uint32_t)tiles, p->target);
     p->bytes = cut ? (uint64_t)p->items * kv_heads * p->rows * (2 + 32ull * nb) * 4 : 0;
@@ -752,17 +811,18 @@ static void att_launch_shape(const AttArgs& a, bool join, dim3 grid, hipStream_t
         hipLaunchKernelGGL((att_kernel<NB, R, kSlot, kPerSimd>), grid, dim3(kAttBlock), 0, s, a);
 }
 
-static void att_launch(const AttArgs& a, const AttPlan& p, bool join, dim3 grid, hipStream_t s) {
-    const int nb = a.c.nb <= 2 ? 2 : a.c.nb <= 4 ? 4 : 8;
-    auto any = [&](auto blocks) {
+// kPerSimd: the waves that a SIMD's registers hold.
+static void att_launch(const AttArgs& a, uint32_t rows, bool join, dim3 grid, hipStream_t s) {
+    auto launch = [&](auto blocks) {
         constexpr int NB = decltype(blocks)::value;
-        if (p.slot == 4) att_launch_shape<NB, 1, 4, NB == 8 ? 2 : 3>(a, join, grid, s);
-        else if (p.slot == 8) att_launch_shape<NB, 1, 8, NB == 8 ? 1 : 2>(a, join, grid, s);
-        else att_launch_shape<NB, NB == 8 ? 1 : 2, 16, NB == 8 ? 1 : 2>(a, join, grid, s);
+        if (rows == 4) att_launch_shape<NB, 1, 4, NB == 8 ? 2 : 3>(a, join, grid, s);
+        else if (rows == 8) att_launch_shape<NB, 1, 8, NB == 8 ? 1 : 2>(a, join, grid, s);
+        else if (rows == 64) att_launch_shape<NB, 1, 16, NB == 8 ? 1 : 2>(a, join, grid, s);
+        else if constexpr (NB < 8) att_launch_shape<NB, 2, 16, 2>(a, join, grid, s);
     };
-    if (nb == 2) any(std::integral_constant<int, 2>());
-    else if (nb == 4) any(std::integral_constant<int, 4>());
-    else any(std::integral_constant<int, 8>());
+    if (a.c.nb <= 2) launch(std::integral_constant<int, 2>());
+    else if (a.c.nb <= 4) launch(std::integral_constant<int, 4>());
+    else launch(std::integral_constant<int, 8>());
 }
 
 static bool att_overlap(const void* a, uint64_t na, const void* b, uint64_t nb) {
@@ -835,7 +895,7 @@ extern "C" int kore_hip_attention_q4_f32(const float* q, const uint8_t* cache, c
     for (int join = 0; join < (p.target ? 2 : 1); ++join) {
         for (a.item0 = 0; a.item0 < p.items; a.item0 += band) {
             const uint32_t x = std::min(band, p.items - a.item0) * (uint32_t)kv_heads;
-            att_launch(a, p, join != 0, dim3(x), (hipStream_t)stream);
+            att_launch(a, p.rows, join != 0, dim3(x), (hipStream_t)stream);
             const int rc = launch_status();
             if (rc != KORE_HIP_OK) return rc;
         }
