@@ -28,7 +28,6 @@ constexpr uint32_t kQkMaxHeadDim = 1024;
 constexpr uint32_t kQkVecHeadDim = 512;  // 64 lanes a row
 constexpr int kQkBlock = 128;
 constexpr int kQkBwBlock = 256;
-constexpr uint32_t kQkBwTile = 8;       // tokens whose cos/sin lie in LDS
 constexpr uint32_t kQkBwParts = 1024;   // partial dw rows at most
 
 struct QkArgs {
@@ -38,13 +37,14 @@ struct QkArgs {
     const float* w[2];
     const float* inv_freq;
     const uint32_t* positions;  // or null: start_pos + token % seq_len
-    float* part;                // backward: [parts][2][D]
+    float* part;                // backward: [parts[0] of q, then parts[1] of k][D]
     uint64_t xs[2], dys[2], ys[2];  // floats between two tokens
     uint64_t tokens, token0, seq_len, start_pos;
     uint32_t heads[2];
     uint32_t dim;
     uint32_t chunks[2];  // forward: workgroups of a token's q and k rows
-    uint32_t tile;       // backward: tokens of a tile
+    uint32_t parts[2];   // backward: workgroups of q, of k
+    uint32_t span;       // backward: tokens that a workgroup's rows may touch
     float eps;
 };
 
@@ -173,85 +173,104 @@ __global__ __launch_bounds__(kQkBwBlock) void qk_norm_rope_any_kernel(QkArgs a) 
     }
 }
 
-// Backward: a workgroup walks tiles of tokens.  A tile's cos/sin go to LDS
-// once; its q rows, then its k rows are dealt to the lane groups.  Each lane
-// keeps the dw of its eight dimensions for q and k over all its rows; the
-// groups' sums meet in LDS at the end and leave as one partial row a workgroup.
-template <int LPR, bool Interleaved>
+// Backward: the rows of Q (or of K), [tokens][heads], are dealt out in runs of one
+// row a lane group, so that the grid sweeps one contiguous band at a time (a
+// workgroup with a run of its own measured 186-205 us where this takes 166).  A
+// run's loads are in flight while the one before it is worked on, and its tokens'
+// cos/sin are computed for it meanwhile.  Each lane keeps the dw of its eight
+// dimensions over all its rows; the groups' sums meet in LDS at the end and leave as
+// one partial row a workgroup.  Whole: all lanes of a group hold values (D = 8 LPR).
+template <int LPR, bool Interleaved, bool Whole>
 __global__ __launch_bounds__(kQkBwBlock) void qk_norm_rope_bwd_kernel(QkArgs a) {
     constexpr uint32_t kGroups = kQkBwBlock / LPR;
-    __shared__ float2 cs[kQkBwTile * LPR * 4];
-    __shared__ float red[kGroups * LPR * 8];
-    const uint32_t l = threadIdx.x % LPR, group = threadIdx.x / LPR, half = a.dim >> 1;
-    const bool ok = l < a.dim >> 3;
+    extern __shared__ f32x4 qk_lds[];  // cos/sin [2][span][D / 2], later sums [groups][D]
+    float2* cs = reinterpret_cast<float2*>(qk_lds);
+    float* red = reinterpret_cast<float*>(qk_lds);
+    const uint32_t lane = threadIdx.x % LPR, group = threadIdx.x / LPR, half = a.dim >> 1;
+    const bool ok = Whole || lane < a.dim >> 3;
+    const uint32_t l = Whole ? lane : min(lane, (a.dim >> 3) - 1);
     const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
-    f32x4 acc[2][2] = {{zero, zero}, {zero, zero}};
-    const uint64_t tiles = (a.tokens + a.tile - 1) / a.tile;
-    for (uint64_t b = blockIdx.x; b < tiles; b += gridDim.x) {
-        const uint64_t t0 = b * a.tile;
-        const uint32_t nt = (uint32_t)(a.tokens - t0 < a.tile ? a.tokens - t0 : a.tile);
-        __syncthreads();
-        for (uint32_t i = threadIdx.x; i < nt * half; i += kQkBwBlock) {
+    const int t = blockIdx.x >= a.parts[0];
+    const uint32_t block = t ? blockIdx.x - a.parts[0] : blockIdx.x;
+    const uint32_t heads = a.heads[t], stride = a.parts[t] * kGroups, rows = (uint32_t)a.tokens * heads;
+    const float* const x = a.x[t];
+    const float* const dy = a.dy[t];
+    float* const y = a.y[t];
+    const uint64_t xs = a.xs[t], dys = a.dys[t], ys = a.ys[t];
+    const f32x4 w0 = ok ? ld4_cached(a.w[t] + 4 * l) : zero, w1 = ok ? ld4_cached(a.w[t] + half + 4 * l) : zero;
+    const float inv_dim = 1.0f / (float)a.dim;
+    f32x4 acc0 = zero, acc1 = zero;
+    auto load = [&](uint32_t run, f32x4 (&o)[4]) {
+        const uint32_t r = min(run + group, rows - 1);  // past the end: a row that is not used
+        const uint32_t tok = r / heads, row = r - tok * heads;
+        const float* p = x + tok * xs + (uint64_t)row * a.dim + 4 * l;
+        const float* d = dy + tok * dys + (uint64_t)row * a.dim + 4 * l;
+        o[0] = ld4(p);
+        o[1] = ld4(p + half);
+        o[2] = ld4(d);
+        o[3] = ld4(d + half);
+    };
+    auto angles = [&](uint32_t run, float2* to) {
+        if (run >= rows) return;
+        const uint32_t first = run / heads, n = (min(run + kGroups, rows) - 1) / heads - first + 1;
+        for (uint32_t i = threadIdx.x; i < n * half; i += kQkBwBlock) {
             const uint32_t tok = i / half, j = i - tok * half;
-            cs[i] = qk_cos_sin(qk_position(a, t0 + tok), a.inv_freq[j]);
+            to[i] = qk_cos_sin(qk_position(a, first + tok), a.inv_freq[j]);
         }
+    };
+    auto work = [&](uint32_t run, const f32x4 (&v)[4], const float2* from) {
+        const uint32_t r = run + group;
+        if (r >= rows) return;
+        const uint32_t tok = r / heads, row = r - tok * heads;
+        float2 c[4];
+        lane_cs<Interleaved>(from + (tok - run / heads) * half, l, a.dim, c);
+        const f32x4 x0 = ok ? v[0] : zero, x1 = ok ? v[1] : zero;
+        f32x4 g0 = ok ? v[2] : zero, g1 = ok ? v[3] : zero;
+        lane_rotate<Interleaved, true>(g0, g1, c);
+        const f32x4 u0 = g0 * w0, u1 = g1 * w1;
+        const float ss = group_sum<LPR>(dot4(x0, x0) + dot4(x1, x1));
+        const float ux = group_sum<LPR>(dot4(u0, x0) + dot4(u1, x1));
+        const float inv = 1.0f / sqrtf(ss / (float)a.dim + a.eps);
+        const f32x4 n0 = x0 * inv, n1 = x1 * inv;
+        acc0 += g0 * n0;
+        acc1 += g1 * n1;
+        const float mean = ux * inv * inv_dim;
+        if (ok) {
+            float* o = y + tok * ys + (uint64_t)row * a.dim + 4 * l;
+            st4(o, (u0 - n0 * mean) * inv);
+            st4(o + half, (u1 - n1 * mean) * inv);
+        }
+    };
+    f32x4 v[2][4];
+    uint32_t run = block * kGroups;
+    load(run, v[0]);
+    angles(run, cs);
+    __syncthreads();
+    for (; run < rows; run += 2 * stride) {
+        load(run + stride, v[1]);
+        angles(run + stride, cs + a.span * half);
+        work(run, v[0], cs);
         __syncthreads();
+        if (run + stride >= rows) break;
+        load(run + 2 * stride, v[0]);
+        angles(run + 2 * stride, cs);
+        work(run + stride, v[1], cs + a.span * half);
+        __syncthreads();
+    }
+    __syncthreads();
+    if (ok) {
+        float* o = red + group * a.dim;
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-            const uint32_t heads = a.heads[t], n = nt * heads;
-            f32x4 w0 = zero, w1 = zero;
-            if (ok && n) {
-                w0 = ld4_cached(a.w[t] + 4 * l);
-                w1 = ld4_cached(a.w[t] + half + 4 * l);
-            }
-            for (uint32_t r = group; r < n; r += kGroups) {
-                const uint32_t tok = r / heads, row = r - tok * heads;
-                const uint64_t token = t0 + tok;
-                f32x4 x0 = zero, x1 = zero, g0 = zero, g1 = zero;
-                float2 c[4] = {};
-                if (ok) {
-                    const float* p = a.x[t] + token * a.xs[t] + (uint64_t)row * a.dim + 4 * l;
-                    const float* d = a.dy[t] + token * a.dys[t] + (uint64_t)row * a.dim + 4 * l;
-                    x0 = ld4(p);
-                    x1 = ld4(p + half);
-                    g0 = ld4(d);
-                    g1 = ld4(d + half);
-                    lane_cs<Interleaved>(cs + tok * half, l, a.dim, c);
-                }
-                lane_rotate<Interleaved, true>(g0, g1, c);
-                const f32x4 u0 = g0 * w0, u1 = g1 * w1;
-                const float ss = group_sum<LPR>(dot4(x0, x0) + dot4(x1, x1));
-                const float ux = group_sum<LPR>(dot4(u0, x0) + dot4(u1, x1));
-                const float inv = 1.0f / sqrtf(ss / (float)a.dim + a.eps);
-                const f32x4 n0 = x0 * inv, n1 = x1 * inv;
-                acc[t][0] += g0 * n0;
-                acc[t][1] += g1 * n1;
-                const float mean = ux * inv / (float)a.dim;
-                if (ok) {
-                    float* o = a.y[t] + token * a.ys[t] + (uint64_t)row * a.dim + 4 * l;
-                    st4(o, (u0 - n0 * mean) * inv);
-                    st4(o + half, (u1 - n1 * mean) * inv);
-                }
-            }
+        for (int j = 0; j < 4; ++j) {
+            o[4 * l + j] = acc0[j];
+            o[half + 4 * l + j] = acc1[j];
         }
     }
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-        __syncthreads();
-        if (ok) {
-            float* o = red + group * a.dim;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                o[4 * l + j] = acc[t][0][j];
-                o[half + 4 * l + j] = acc[t][1][j];
-            }
-        }
-        __syncthreads();
-        for (uint32_t d = threadIdx.x; d < a.dim; d += kQkBwBlock) {
-            float s = 0.0f;
-            for (uint32_t g = 0; g < kGroups; ++g) s += red[g * a.dim + d];
-            a.part[((uint64_t)blockIdx.x * 2 + t) * a.dim + d] = s;
-        }
+    __syncthreads();
+    for (uint32_t d = threadIdx.x; d < a.dim; d += kQkBwBlock) {
+        float s = 0.0f;
+        for (uint32_t g = 0; g < kGroups; ++g) s += red[g * a.dim + d];
+        a.part[(uint64_t)blockIdx.x * a.dim + d] = s;
     }
 }
 
@@ -260,74 +279,73 @@ __global__ __launch_bounds__(kQkBwBlock) void qk_norm_rope_bwd_kernel(QkArgs a) 
 template <bool Interleaved>
 __global__ __launch_bounds__(kQkBwBlock) void qk_norm_rope_bwd_any_kernel(QkArgs a) {
     constexpr uint32_t kWaves = kQkBwBlock / kWave;
-    extern __shared__ float dw[];  // [kWaves][2][D]
+    extern __shared__ f32x4 qk_lds[];
+    float* dw = reinterpret_cast<float*>(qk_lds);  // [kWaves][D]
     const uint32_t wave = threadIdx.x / kWave, lane = threadIdx.x % kWave, half = a.dim >> 1;
-    const uint32_t heads = a.heads[0] + a.heads[1];
-    for (uint32_t i = threadIdx.x; i < kWaves * 2 * a.dim; i += kQkBwBlock) dw[i] = 0.0f;
+    const int t = blockIdx.x >= a.parts[0];
+    const uint32_t block = t ? blockIdx.x - a.parts[0] : blockIdx.x;
+    const uint32_t heads = a.heads[t], rows = (uint32_t)a.tokens * heads;
+    for (uint32_t i = threadIdx.x; i < kWaves * a.dim; i += kQkBwBlock) dw[i] = 0.0f;
     __syncthreads();
-    const uint64_t tiles = (a.tokens + a.tile - 1) / a.tile;
-    for (uint64_t b = blockIdx.x; b < tiles; b += gridDim.x) {
-        const uint64_t t0 = b * a.tile;
-        const uint32_t nt = (uint32_t)(a.tokens - t0 < a.tile ? a.tokens - t0 : a.tile);
-        for (uint32_t r = wave; r < nt * heads; r += kWaves) {
-            const uint64_t token = t0 + r / heads;
-            uint32_t row = r % heads;
-            const int t = row >= a.heads[0];
-            if (t) row -= a.heads[0];
-            const float* x = a.x[t] + token * a.xs[t] + (uint64_t)row * a.dim;
-            const float* dy = a.dy[t] + token * a.dys[t] + (uint64_t)row * a.dim;
-            float* y = a.y[t] + token * a.ys[t] + (uint64_t)row * a.dim;
-            const float* w = a.w[t];
-            float* mine = dw + (wave * 2 + t) * a.dim;
-            const uint64_t pos = qk_position(a, token);
-            float ss = 0.0f, ux = 0.0f;
-            for (uint32_t i = lane; i < half; i += kWave) {
-                const uint32_t j0 = Interleaved ? 2 * i : i, j1 = Interleaved ? 2 * i + 1 : i + half;
-                const float2 c = qk_cos_sin(pos, a.inv_freq[i]);
-                const float g0 = __builtin_fmaf(dy[j0], c.x, dy[j1] * c.y), g1 = __builtin_fmaf(dy[j1], c.x, -(dy[j0] * c.y));
-                ss += __builtin_fmaf(x[j0], x[j0], x[j1] * x[j1]);
-                ux += __builtin_fmaf(g0 * w[j0], x[j0], g1 * w[j1] * x[j1]);
-            }
-            ss = group_sum<kWave>(ss);
-            ux = group_sum<kWave>(ux);
-            const float inv = 1.0f / sqrtf(ss / (float)a.dim + a.eps);
-            const float mean = ux * inv / (float)a.dim;
-            for (uint32_t i = lane; i < half; i += kWave) {
-                const uint32_t j0 = Interleaved ? 2 * i : i, j1 = Interleaved ? 2 * i + 1 : i + half;
-                const float2 c = qk_cos_sin(pos, a.inv_freq[i]);
-                const float g0 = __builtin_fmaf(dy[j0], c.x, dy[j1] * c.y), g1 = __builtin_fmaf(dy[j1], c.x, -(dy[j0] * c.y));
-                const float n0 = x[j0] * inv, n1 = x[j1] * inv;
-                mine[j0] += g0 * n0;
-                mine[j1] += g1 * n1;
-                y[j0] = (g0 * w[j0] - n0 * mean) * inv;
-                y[j1] = (g1 * w[j1] - n1 * mean) * inv;
-            }
+    float* mine = dw + wave * a.dim;
+    const float* w = a.w[t];
+    for (uint32_t r = block * kWaves + wave; r < rows; r += a.parts[t] * kWaves) {
+        const uint32_t token = r / heads, row = r - token * heads;
+        const float* x = a.x[t] + token * a.xs[t] + (uint64_t)row * a.dim;
+        const float* dy = a.dy[t] + token * a.dys[t] + (uint64_t)row * a.dim;
+        float* y = a.y[t] + token * a.ys[t] + (uint64_t)row * a.dim;
+        const uint64_t pos = qk_position(a, token);
+        float ss = 0.0f, ux = 0.0f;
+        for (uint32_t i = lane; i < half; i += kWave) {
+            const uint32_t j0 = Interleaved ? 2 * i : i, j1 = Interleaved ? 2 * i + 1 : i + half;
+            const float2 c = qk_cos_sin(pos, a.inv_freq[i]);
+            const float g0 = __builtin_fmaf(dy[j0], c.x, dy[j1] * c.y), g1 = __builtin_fmaf(dy[j1], c.x, -(dy[j0] * c.y));
+            ss += __builtin_fmaf(x[j0], x[j0], x[j1] * x[j1]);
+            ux += __builtin_fmaf(g0 * w[j0], x[j0], g1 * w[j1] * x[j1]);
+        }
+        ss = group_sum<kWave>(ss);
+        ux = group_sum<kWave>(ux);
+        const float inv = 1.0f / sqrtf(ss / (float)a.dim + a.eps);
+        const float mean = ux * inv / (float)a.dim;
+        for (uint32_t i = lane; i < half; i += kWave) {
+            const uint32_t j0 = Interleaved ? 2 * i : i, j1 = Interleaved ? 2 * i + 1 : i + half;
+            const float2 c = qk_cos_sin(pos, a.inv_freq[i]);
+            const float g0 = __builtin_fmaf(dy[j0], c.x, dy[j1] * c.y), g1 = __builtin_fmaf(dy[j1], c.x, -(dy[j0] * c.y));
+            const float n0 = x[j0] * inv, n1 = x[j1] * inv;
+            mine[j0] += g0 * n0;
+            mine[j1] += g1 * n1;
+            y[j0] = (g0 * w[j0] - n0 * mean) * inv;
+            y[j1] = (g1 * w[j1] - n1 * mean) * inv;
         }
     }
     __syncthreads();
-    for (uint32_t d = threadIdx.x; d < 2 * a.dim; d += kQkBwBlock) {
+    for (uint32_t d = threadIdx.x; d < a.dim; d += kQkBwBlock) {
         float s = 0.0f;
-        for (uint32_t v = 0; v < kWaves; ++v) s += dw[v * 2 * a.dim + d];
-        a.part[(uint64_t)blockIdx.x * 2 * a.dim + d] = s;
+        for (uint32_t v = 0; v < kWaves; ++v) s += dw[v * a.dim + d];
+        a.part[(uint64_t)blockIdx.x * a.dim + d] = s;
     }
 }
 
 // dw[t][d] = the partial rows' sum, in a fixed order: 64 row slots a column, eight
 // rows of a slot in flight.
 constexpr int kQkRedCols = 16, kQkRedSlots = 64, kQkRedFlight = 8;
-__global__ __launch_bounds__(kQkRedCols* kQkRedSlots) void qk_norm_rope_dw_kernel(const float* part, uint32_t parts,
-                                                                                  uint32_t dim, float* dqw, float* dkw) {
+__global__ __launch_bounds__(kQkRedCols* kQkRedSlots) void qk_norm_rope_dw_kernel(const float* part, uint32_t q_parts,
+                                                                                  uint32_t k_parts, uint32_t dim,
+                                                                                  float* dqw, float* dkw) {
     __shared__ float red[kQkRedSlots][kQkRedCols + 1];
     const uint32_t c = threadIdx.x % kQkRedCols, slot = threadIdx.x / kQkRedCols;
     const uint32_t col = blockIdx.x * kQkRedCols + c;
+    const int t = blockIdx.y;  // 0: q, 1: k
+    const uint32_t parts = t ? k_parts : q_parts;
+    if (t) part += (uint64_t)q_parts * dim;
     float s = 0.0f;
-    if (col < 2 * dim) {
+    if (col < dim) {
         for (uint32_t p = slot; p < parts; p += kQkRedSlots * kQkRedFlight) {
             float v[kQkRedFlight];
 #pragma unroll
             for (int i = 0; i < kQkRedFlight; ++i) {
                 const uint32_t at = p + i * kQkRedSlots;
-                v[i] = at < parts ? part[(uint64_t)at * 2 * dim + col] : 0.0f;
+                v[i] = at < parts ? part[(uint64_t)at * dim + col] : 0.0f;
             }
 #pragma unroll
             for (int i = 0; i < kQkRedFlight; ++i) s += v[i];
@@ -340,9 +358,8 @@ __global__ __launch_bounds__(kQkRedCols* kQkRedSlots) void qk_norm_rope_dw_kerne
         if (slot < (uint32_t)n) red[slot][c] += red[slot + n][c];
         __syncthreads();
     }
-    if (slot || col >= 2 * dim) return;
-    float* o = col < dim ? dqw : dkw;
-    if (o) o[col < dim ? col : col - dim] = red[0][c];
+    float* o = t ? dkw : dqw;
+    if (slot == 0 && col < dim && o) o[col] = red[0][c];
 }
 
 // Whether rows of `wa` floats every `sa` from a meet rows of `wb` every `sb`
@@ -357,17 +374,29 @@ static bool rows_overlap(const float* a, uint64_t sa, uint64_t wa, const float* 
     return off < wa || off + wb > sa;
 }
 
+static uint32_t qk_lanes(uint32_t dim) {
+    uint32_t l = 1;
+    while (l * 8 < dim) l *= 2;
+    return l;
+}
+
+static bool qk_vector(uint32_t dim) { return dim % 8 == 0 && dim <= kQkVecHeadDim; }
+
 struct QkPlan {
-    uint32_t tile;   // tokens
-    uint32_t parts;  // workgroups, each a partial dw row
+    uint32_t parts[2];  // workgroups of q and k, each a partial dw row
+    uint32_t groups;    // rows of a run
 };
 
-// Tiles of up to eight tokens once there are enough of them for 1024
-// workgroups, which then share the tiles.
-static QkPlan qk_plan(uint64_t tokens) {
-    const uint32_t tile = (uint32_t)std::min<uint64_t>(kQkBwTile, std::max<uint64_t>(1, tokens / kQkBwParts));
-    const uint64_t tiles = (tokens + tile - 1) / tile;
-    return {tile, (uint32_t)std::min<uint64_t>(tiles, kQkBwParts)};
+// 1024 workgroups, four to a CU, shared out as Q's and K's heads are.
+static QkPlan qk_plan(uint64_t tokens, uint32_t q_heads, uint32_t k_heads, uint32_t dim) {
+    QkPlan p = {};
+    p.groups = kQkBwBlock / (qk_vector(dim) ? qk_lanes(dim) : kWave);
+    const uint32_t heads[2] = {q_heads, k_heads};
+    for (int t = 0; t < 2; ++t) {
+        const uint64_t share = (uint64_t)kQkBwParts * heads[t] / ((uint64_t)q_heads + k_heads);
+        p.parts[t] = (uint32_t)std::min((tokens * heads[t] + p.groups - 1) / p.groups, std::max<uint64_t>(share, 1));
+    }
+    return p;
 }
 
 // Checks shared by both directions; fills dims, strides and the launch's tokens.
@@ -414,12 +443,6 @@ static bool qk_outputs_alias(const QkArgs& a) {
                         (uint64_t)a.heads[1] * a.dim, a.tokens);
 }
 
-static uint32_t qk_lanes(uint32_t dim) {
-    uint32_t l = 1;
-    while (l * 8 < dim) l *= 2;
-    return l;
-}
-
 #define QK_LANES(L, CALL)                  \
     switch (L) {                           \
         case 1: { CALL(1); } break;        \
@@ -462,7 +485,7 @@ extern "C" int kore_hip_qk_norm_rope_f32(const float* q, const float* k, const f
     a.eps = eps;
     if (qk_alias(a, a.x, a.xs, true) || qk_outputs_alias(a)) return KORE_HIP_ERR_ALIAS;
     hipStream_t s = (hipStream_t)stream;
-    const bool vec = head_dim % 8 == 0 && head_dim <= kQkVecHeadDim;
+    const bool vec = qk_vector(head_dim);
     const uint32_t lanes = qk_lanes(head_dim), rows = kQkBlock / std::min(lanes, 64u);
     a.chunks[0] = (q_heads + rows - 1) / rows;
     a.chunks[1] = (k_heads + rows - 1) / rows;
@@ -500,7 +523,8 @@ extern "C" int kore_hip_qk_norm_rope_f32(const float* q, const float* k, const f
 extern "C" uint64_t kore_hip_qk_norm_rope_backward_workspace_bytes(uint64_t tokens, uint32_t q_heads, uint32_t k_heads,
                                                                    uint32_t head_dim) {
     if (tokens == 0 || head_dim == 0 || head_dim > kQkMaxHeadDim || (q_heads == 0 && k_heads == 0)) return 0;
-    return (uint64_t)qk_plan(tokens).parts * 2 * head_dim * sizeof(float);
+    const QkPlan p = qk_plan(tokens, q_heads, k_heads, head_dim);
+    return ((uint64_t)p.parts[0] + p.parts[1]) * head_dim * sizeof(float);
 }
 
 extern "C" int kore_hip_qk_norm_rope_backward_f32(
@@ -522,9 +546,11 @@ extern "C" int kore_hip_qk_norm_rope_backward_f32(
     const int st = qk_check(&a, batch, seq_len, q_heads, k_heads, head_dim, start_pos, positions);
     if (st != KORE_HIP_OK) return st;
     if ((q_heads && !grad_q_weight) || (k_heads && !grad_k_weight)) return KORE_HIP_ERR_NULL_PTR;
+    // rows are counted in 32 bits, with room for a sweep of the grid
+    if (a.tokens * std::max(q_heads, k_heads) > 0xf0000000ull) return KORE_HIP_ERR_OVERFLOW;
     const uint64_t need = kore_hip_qk_norm_rope_backward_workspace_bytes(a.tokens, q_heads, k_heads, head_dim);
     hipStream_t s = (hipStream_t)stream;
-    const QkPlan plan = qk_plan(a.tokens);
+    const QkPlan plan = qk_plan(a.tokens, q_heads, k_heads, head_dim);
     if (a.tokens) {
         if (!inv_freq || !workspace || (q_heads && (!grad_q_out || !q || !q_weight || !grad_q)) ||
             (k_heads && (!grad_k_out || !k || !k_weight || !grad_k)))
@@ -541,26 +567,33 @@ extern "C" int kore_hip_qk_norm_rope_backward_f32(
         a.inv_freq = inv_freq;
         a.eps = eps;
         a.part = workspace;
-        a.tile = plan.tile;
+        for (int t = 0; t < 2; ++t) a.parts[t] = plan.parts[t];
         if (qk_alias(a, a.x, a.xs, true) || qk_alias(a, a.dy, a.dys, true) || qk_outputs_alias(a))
             return KORE_HIP_ERR_ALIAS;
-        const dim3 grid(plan.parts), block(kQkBwBlock);
-        if (head_dim % 8 == 0 && head_dim <= kQkVecHeadDim) {
-#define QK_CALL(L)                                                                                            \
-    if (interleaved) hipLaunchKernelGGL((qk_norm_rope_bwd_kernel<L, true>), grid, block, 0, s, a);            \
-    else hipLaunchKernelGGL((qk_norm_rope_bwd_kernel<L, false>), grid, block, 0, s, a);
-            QK_LANES(qk_lanes(head_dim), QK_CALL)
+        const dim3 grid(plan.parts[0] + plan.parts[1]), block(kQkBwBlock);
+        if (qk_vector(head_dim)) {
+            const uint32_t lanes = qk_lanes(head_dim);
+            const uint32_t fewest = !q_heads ? k_heads : !k_heads ? q_heads : std::min(q_heads, k_heads);
+            a.span = (plan.groups - 1) / fewest + 2;
+            const size_t lds = (size_t)std::max(2 * a.span, plan.groups) * head_dim * sizeof(float);
+            const bool whole = head_dim == 8 * lanes;
+#define QK_CALL(L)                                                                                                       \
+    if (interleaved && whole) hipLaunchKernelGGL((qk_norm_rope_bwd_kernel<L, true, true>), grid, block, lds, s, a);      \
+    else if (interleaved) hipLaunchKernelGGL((qk_norm_rope_bwd_kernel<L, true, false>), grid, block, lds, s, a);         \
+    else if (whole) hipLaunchKernelGGL((qk_norm_rope_bwd_kernel<L, false, true>), grid, block, lds, s, a);               \
+    else hipLaunchKernelGGL((qk_norm_rope_bwd_kernel<L, false, false>), grid, block, lds, s, a);
+            QK_LANES(lanes, QK_CALL)
 #undef QK_CALL
         } else {
-            const size_t lds = (size_t)(kQkBwBlock / kWave) * 2 * head_dim * sizeof(float);
+            const size_t lds = (size_t)(kQkBwBlock / kWave) * head_dim * sizeof(float);
             if (interleaved) hipLaunchKernelGGL(qk_norm_rope_bwd_any_kernel<true>, grid, block, lds, s, a);
             else hipLaunchKernelGGL(qk_norm_rope_bwd_any_kernel<false>, grid, block, lds, s, a);
         }
         const int rc = launch_status();
         if (rc != KORE_HIP_OK) return rc;
     }
-    hipLaunchKernelGGL(qk_norm_rope_dw_kernel, dim3((2 * head_dim + kQkRedCols - 1) / kQkRedCols),
-                       dim3(kQkRedCols * kQkRedSlots), 0, s, workspace, a.tokens ? plan.parts : 0u, head_dim, q_heads ? grad_q_weight : nullptr,
-                       k_heads ? grad_k_weight : nullptr);
+    hipLaunchKernelGGL(qk_norm_rope_dw_kernel, dim3((head_dim + kQkRedCols - 1) / kQkRedCols, 2),
+                       dim3(kQkRedCols * kQkRedSlots), 0, s, workspace, plan.parts[0], plan.parts[1], head_dim,
+                       q_heads ? grad_q_weight : nullptr, k_heads ? grad_k_weight : nullptr);
     return launch_status();
 }

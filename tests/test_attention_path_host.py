@@ -124,9 +124,10 @@ def test_norm_rope_backward_refusals():
         assert norm_rope_bwd(strides=s) == DIM, i
     assert norm_rope_bwd(gq=P + 5 * M + 4) == ALIAS and norm_rope_bwd(gq=P + M) == ALIAS and norm_rope_bwd(gk=P + 2 * M) == ALIAS
     assert norm_rope_bwd(gq=P + 4) == ALIAS
+    assert norm_rope_bwd(batch=2 ** 30, seq=1, wsb=2 ** 40) == OVER  # more than 32 bits of rows
     ws = lib.kore_hip_qk_norm_rope_backward_workspace_bytes
-    assert ws(0, 4, 2, 64) == 0 and ws(5, 0, 0, 64) == 0 and ws(1, 1, 1, 64) == 512
-    assert ws(2 ** 30, 32, 8, 128) == 1024 * 2 * 128 * 4
+    assert ws(0, 4, 2, 64) == 0 and ws(5, 0, 0, 64) == 0 and ws(1, 1, 1, 64) == 512 and ws(1, 3, 0, 64) == 256
+    assert ws(2 ** 30, 32, 8, 128) == 1023 * 128 * 4 and ws(20, 2, 1, 128) == 5 * 128 * 4
 
 
 def cache_write(k=P, v=P + M, slots=P + 2 * M, cache=P + 3 * M, tokens=5, heads=2, d=64, pages=4, page=16, ks=0, vs=0):
