@@ -509,9 +509,18 @@ __all__ += ["rocm_ternary_matmul_i8", "rocm_ternary_matmul_f32", "rocm_bit_linea
 
 
 # ------------------------------------------- query/key norm with rotation
-def _rows(tokens: int, stride: int, row: int) -> int:
+# These ops take many buffers, and a decode step calls each of them a layer: sizes
+# are compared in one expression and only a failure looks for the buffer to name
+# (qk_norm_rope on one token 6.7 -> 5.2 us of host time).
+def _span(tokens: int, stride: int, row: int) -> int:
     """Bytes from a token's first float to the last token's end (stride 0: contiguous rows)."""
     return ((tokens - 1) * (stride or row) + row) * 4 if tokens and row else 0
+
+
+def _needs(op: str, *named) -> None:
+    """Raises for the first (name, buffer, bytes) that is too small."""
+    for name, buf, nbytes in named:
+        _need(buf, nbytes, op, name)
 
 
 def rocm_qk_norm_rope_f32(device_idx: int, q: HipBuffer, k: HipBuffer, q_weight: HipBuffer, k_weight: HipBuffer,
@@ -527,22 +536,27 @@ def rocm_qk_norm_rope_f32(device_idx: int, q: HipBuffer, k: HipBuffer, q_weight:
     token) replaces ``start_pos + s``.  Returns (q_out, k_out); q and k
     themselves may be given for in-place work."""
     lib = _library(device_idx)
-    t = batch * seq_len
-    _need(q, _rows(t, q_stride, q_heads * head_dim), "qk_norm_rope q")
-    _need(k, _rows(t, k_stride, k_heads * head_dim), "qk_norm_rope k")
-    _need(q_weight, head_dim * 4 if q_heads else 0, "qk_norm_rope q_weight")
-    _need(k_weight, head_dim * 4 if k_heads else 0, "qk_norm_rope k_weight")
-    _need(inv_freq, (head_dim // 2) * 4, "qk_norm_rope inv_freq")
-    if positions is not None:
-        _need(positions, t * 4, "qk_norm_rope positions")
-    qo = _out(device_idx, q_out, _rows(t, q_out_stride, q_heads * head_dim), "qk_norm_rope q_out")
-    ko = _out(device_idx, k_out, _rows(t, k_out_stride, k_heads * head_dim), "qk_norm_rope k_out")
-    _check(lib.kore_hip_qk_norm_rope_f32(q.ptr, k.ptr, q_weight.ptr, k_weight.ptr, inv_freq.ptr,
-                                         positions.ptr if positions is not None else None, qo.ptr, ko.ptr, batch,
-                                         seq_len, q_heads, k_heads, head_dim, q_stride, k_stride, q_out_stride,
-                                         k_out_stride, start_pos, eps, int(bool(interleaved)), _stream(device_idx)),
-           "qk_norm_rope_f32")
-    return qo, ko
+    t, rq, rk, w = batch * seq_len, q_heads * head_dim, k_heads * head_dim, head_dim * 4
+    nqo, nko = _span(t, q_out_stride, rq), _span(t, k_out_stride, rk)
+    if q_out is None:
+        q_out = HipBuffer.empty(device_idx, nqo)
+    if k_out is None:
+        k_out = HipBuffer.empty(device_idx, nko)
+    qt, kt, qwt, kwt, ft, qot, kot = q._t, k._t, q_weight._t, k_weight._t, inv_freq._t, q_out._t, k_out._t
+    nq, nk = _span(t, q_stride, rq), _span(t, k_stride, rk)
+    if (qt.numel() < nq or kt.numel() < nk or qwt.numel() < w or kwt.numel() < w or ft.numel() < w // 8 * 4
+            or qot.numel() < nqo or kot.numel() < nko or (positions is not None and positions._t.numel() < t * 4)):
+        _needs("qk_norm_rope", ("q", q, nq), ("k", k, nk), ("q_weight", q_weight, w if rq else 0),
+               ("k_weight", k_weight, w if rk else 0), ("inv_freq", inv_freq, w // 8 * 4), ("q_out", q_out, nqo),
+               ("k_out", k_out, nko), ("positions", positions or q, t * 4 if positions else 0))
+    status = lib.kore_hip_qk_norm_rope_f32(
+        qt.data_ptr(), kt.data_ptr(), qwt.data_ptr(), kwt.data_ptr(), ft.data_ptr(),
+        None if positions is None else positions._t.data_ptr(), qot.data_ptr(), kot.data_ptr(), batch, seq_len, q_heads,
+        k_heads, head_dim, q_stride, k_stride, q_out_stride, k_out_stride, start_pos, eps, 1 if interleaved else 0,
+        _stream(device_idx))
+    if status:
+        _check(status, "qk_norm_rope_f32")
+    return q_out, k_out
 
 
 def rocm_qk_norm_rope_backward_workspace_bytes(tokens: int, q_heads: int, k_heads: int, head_dim: int) -> int:
@@ -562,32 +576,43 @@ def rocm_qk_norm_rope_backward_f32(device_idx: int, grad_q_out: HipBuffer, grad_
     """Backward of ``rocm_qk_norm_rope_f32`` -> (grad_q, grad_k,
     grad_q_weight, grad_k_weight).  The workspace is allocated when not given."""
     lib = _library(device_idx)
-    t = batch * seq_len
-    rq, rk = q_heads * head_dim, k_heads * head_dim
-    _need(grad_q_out, _rows(t, grad_q_out_stride, rq), "qk_norm_rope_backward grad_q_out")
-    _need(grad_k_out, _rows(t, grad_k_out_stride, rk), "qk_norm_rope_backward grad_k_out")
-    _need(q, _rows(t, q_stride, rq), "qk_norm_rope_backward q")
-    _need(k, _rows(t, k_stride, rk), "qk_norm_rope_backward k")
-    _need(q_weight, head_dim * 4 if q_heads else 0, "qk_norm_rope_backward q_weight")
-    _need(k_weight, head_dim * 4 if k_heads else 0, "qk_norm_rope_backward k_weight")
-    _need(inv_freq, (head_dim // 2) * 4, "qk_norm_rope_backward inv_freq")
-    if positions is not None:
-        _need(positions, t * 4, "qk_norm_rope_backward positions")
-    gq = _out(device_idx, grad_q, _rows(t, grad_q_stride, rq), "qk_norm_rope_backward grad_q")
-    gk = _out(device_idx, grad_k, _rows(t, grad_k_stride, rk), "qk_norm_rope_backward grad_k")
-    gqw = _out(device_idx, grad_q_weight, head_dim * 4 if q_heads else 0, "qk_norm_rope_backward grad_q_weight")
-    gkw = _out(device_idx, grad_k_weight, head_dim * 4 if k_heads else 0, "qk_norm_rope_backward grad_k_weight")
-    ws = workspace if workspace is not None else HipBuffer.empty(device_idx, max(
-        16, rocm_qk_norm_rope_backward_workspace_bytes(t, q_heads, k_heads, head_dim)))
-    _check(lib.kore_hip_qk_norm_rope_backward_f32(
-        grad_q_out.ptr, grad_k_out.ptr, q.ptr, k.ptr, q_weight.ptr, k_weight.ptr, inv_freq.ptr,
-        positions.ptr if positions is not None else None, gq.ptr, gk.ptr, gqw.ptr, gkw.ptr, ws.ptr, ws.nbytes, batch,
-        seq_len, q_heads, k_heads, head_dim, grad_q_out_stride, grad_k_out_stride, q_stride, k_stride, grad_q_stride,
-        grad_k_stride, start_pos, eps, int(bool(interleaved)), _stream(device_idx)), "qk_norm_rope_backward_f32")
+    t, rq, rk, w = batch * seq_len, q_heads * head_dim, k_heads * head_dim, head_dim * 4
+    ngq, ngk = _span(t, grad_q_stride, rq), _span(t, grad_k_stride, rk)
+    gq = HipBuffer.empty(device_idx, ngq) if grad_q is None else grad_q
+    gk = HipBuffer.empty(device_idx, ngk) if grad_k is None else grad_k
+    gqw = HipBuffer.empty(device_idx, w) if grad_q_weight is None else grad_q_weight
+    gkw = HipBuffer.empty(device_idx, w) if grad_k_weight is None else grad_k_weight
+    if workspace is None:
+        workspace = HipBuffer.empty(device_idx, max(16, rocm_qk_norm_rope_backward_workspace_bytes(
+            t, q_heads, k_heads, head_dim)))
+    nq, nk = _span(t, q_stride, rq), _span(t, k_stride, rk)
+    ndq, ndk = _span(t, grad_q_out_stride, rq), _span(t, grad_k_out_stride, rk)
+    dqt, dkt, qt, kt, qwt, kwt, ft = (grad_q_out._t, grad_k_out._t, q._t, k._t, q_weight._t, k_weight._t, inv_freq._t)
+    gqt, gkt, gqwt, gkwt, wst = gq._t, gk._t, gqw._t, gkw._t, workspace._t
+    if (qt.numel() < nq or kt.numel() < nk or dqt.numel() < ndq or dkt.numel() < ndk or qwt.numel() < w
+            or kwt.numel() < w or ft.numel() < w // 8 * 4 or gqt.numel() < ngq or gkt.numel() < ngk
+            or gqwt.numel() < w or gkwt.numel() < w or (positions is not None and positions._t.numel() < t * 4)):
+        _needs("qk_norm_rope_backward", ("grad_q_out", grad_q_out, ndq), ("grad_k_out", grad_k_out, ndk), ("q", q, nq),
+               ("k", k, nk), ("q_weight", q_weight, w if rq else 0), ("k_weight", k_weight, w if rk else 0),
+               ("inv_freq", inv_freq, w // 8 * 4), ("grad_q", gq, ngq), ("grad_k", gk, ngk),
+               ("grad_q_weight", gqw, w if rq else 0), ("grad_k_weight", gkw, w if rk else 0),
+               ("positions", positions or q, t * 4 if positions else 0))
+    status = lib.kore_hip_qk_norm_rope_backward_f32(
+        dqt.data_ptr(), dkt.data_ptr(), qt.data_ptr(), kt.data_ptr(), qwt.data_ptr(), kwt.data_ptr(), ft.data_ptr(),
+        None if positions is None else positions._t.data_ptr(), gqt.data_ptr(), gkt.data_ptr(), gqwt.data_ptr(),
+        gkwt.data_ptr(), wst.data_ptr(), wst.numel(), batch, seq_len, q_heads, k_heads, head_dim, grad_q_out_stride,
+        grad_k_out_stride, q_stride, k_stride, grad_q_stride, grad_k_stride, start_pos, eps, 1 if interleaved else 0,
+        _stream(device_idx))
+    if status:
+        _check(status, "qk_norm_rope_backward_f32")
     return gq, gk, gqw, gkw
 
 
 # --------------------------------------------------- 4-bit key/value cache
+def _cache_bytes(num_pages: int, page_size: int, kv_heads: int, head_dim: int) -> int:
+    return num_pages * page_size * kv_heads * ((head_dim + 31) // 32) * 34
+
+
 def rocm_kv_cache_q4_bytes(num_pages: int, page_size: int, kv_heads: int, head_dim: int) -> int:
     """Size of one layer's 4-bit cache (include/kore_hip.h has its layout)."""
     n = int(_lib.load().kore_hip_kv_cache_q4_bytes(num_pages, page_size, kv_heads, head_dim))
@@ -606,13 +631,15 @@ def rocm_kv_cache_write_q4_f32(device_idx: int, k: HipBuffer, v: HipBuffer, slot
     f32 there)."""
     lib = _library(device_idx)
     row = kv_heads * head_dim
-    _need(k, _rows(tokens, k_stride, row), "kv_cache_write k")
-    _need(v, _rows(tokens, v_stride, row), "kv_cache_write v")
-    _need(slots, tokens * 4, "kv_cache_write slots")
-    _need(cache, lib.kore_hip_kv_cache_q4_bytes(num_pages, page_size, kv_heads, head_dim), "kv_cache_write cache")
-    _check(lib.kore_hip_kv_cache_write_q4_f32(k.ptr, v.ptr, slots.ptr, cache.ptr, tokens, kv_heads, head_dim,
-                                              num_pages, page_size, k_stride, v_stride, _stream(device_idx)),
-           "kv_cache_write_q4_f32")
+    nk, nv, nc = _span(tokens, k_stride, row), _span(tokens, v_stride, row), _cache_bytes(num_pages, page_size, kv_heads, head_dim)
+    kt, vt, st, ct = k._t, v._t, slots._t, cache._t
+    if kt.numel() < nk or vt.numel() < nv or st.numel() < tokens * 4 or ct.numel() < nc:
+        _needs("kv_cache_write", ("k", k, nk), ("v", v, nv), ("slots", slots, tokens * 4), ("cache", cache, nc))
+    status = lib.kore_hip_kv_cache_write_q4_f32(kt.data_ptr(), vt.data_ptr(), st.data_ptr(), ct.data_ptr(), tokens,
+                                                kv_heads, head_dim, num_pages, page_size, k_stride, v_stride,
+                                                _stream(device_idx))
+    if status:
+        _check(status, "kv_cache_write_q4_f32")
 
 
 def rocm_kv_cache_read_q4_f32(device_idx: int, cache: HipBuffer, slots: HipBuffer, tokens: int, kv_heads: int,
@@ -620,14 +647,19 @@ def rocm_kv_cache_read_q4_f32(device_idx: int, cache: HipBuffer, slots: HipBuffe
                               v_out: Optional[HipBuffer] = None) -> Tuple[HipBuffer, HipBuffer]:
     """The cached values of ``tokens`` slots as f32 (k, v) [tokens, kv_heads, head_dim]."""
     lib = _library(device_idx)
-    n = tokens * kv_heads * head_dim * 4
-    _need(slots, tokens * 4, "kv_cache_read slots")
-    _need(cache, lib.kore_hip_kv_cache_q4_bytes(num_pages, page_size, kv_heads, head_dim), "kv_cache_read cache")
-    ko = _out(device_idx, k_out, n, "kv_cache_read k_out")
-    vo = _out(device_idx, v_out, n, "kv_cache_read v_out")
-    _check(lib.kore_hip_kv_cache_read_q4_f32(cache.ptr, slots.ptr, ko.ptr, vo.ptr, tokens, kv_heads, head_dim,
-                                             num_pages, page_size, _stream(device_idx)), "kv_cache_read_q4_f32")
-    return ko, vo
+    n, nc = tokens * kv_heads * head_dim * 4, _cache_bytes(num_pages, page_size, kv_heads, head_dim)
+    if k_out is None:
+        k_out = HipBuffer.empty(device_idx, n)
+    if v_out is None:
+        v_out = HipBuffer.empty(device_idx, n)
+    ct, st, kt, vt = cache._t, slots._t, k_out._t, v_out._t
+    if kt.numel() < n or vt.numel() < n or st.numel() < tokens * 4 or ct.numel() < nc:
+        _needs("kv_cache_read", ("slots", slots, tokens * 4), ("cache", cache, nc), ("k_out", k_out, n), ("v_out", v_out, n))
+    status = lib.kore_hip_kv_cache_read_q4_f32(ct.data_ptr(), st.data_ptr(), kt.data_ptr(), vt.data_ptr(), tokens,
+                                               kv_heads, head_dim, num_pages, page_size, _stream(device_idx))
+    if status:
+        _check(status, "kv_cache_read_q4_f32")
+    return k_out, v_out
 
 
 def rocm_attention_q4_workspace_bytes(num_seqs: int, tokens: int, q_heads: int, kv_heads: int, head_dim: int,
@@ -651,20 +683,25 @@ def rocm_attention_q4_f32(device_idx: int, q: HipBuffer, cache: HipBuffer, page_
     The workspace is allocated when not given."""
     lib = _library(device_idx)
     row = q_heads * head_dim
-    _need(q, _rows(tokens, q_stride, row), "attention q")
-    _need(cache, lib.kore_hip_kv_cache_q4_bytes(num_pages, page_size, kv_heads, head_dim), "attention cache")
-    _need(page_table, num_seqs * max_pages * 4, "attention page_table")
-    _need(kv_lens, num_seqs * 4, "attention kv_lens")
-    _need(q_starts, (num_seqs + 1) * 4 if num_seqs else 0, "attention q_starts")
-    o = _out(device_idx, out, tokens * row * 4, "attention out")
+    nq, no = _span(tokens, q_stride, row), tokens * row * 4
+    nc, ns = _cache_bytes(num_pages, page_size, kv_heads, head_dim), num_seqs * 4 + 4 if num_seqs else 0
+    if out is None:
+        out = HipBuffer.empty(device_idx, no)
     if workspace is None:
         workspace = HipBuffer.empty(device_idx, max(16, lib.kore_hip_attention_q4_workspace_bytes(
             num_seqs, tokens, q_heads, kv_heads, head_dim, page_size, max_pages)))
-    _check(lib.kore_hip_attention_q4_f32(q.ptr, cache.ptr, page_table.ptr, kv_lens.ptr, q_starts.ptr, o.ptr,
-                                         workspace.ptr, workspace.nbytes, num_seqs, tokens, q_heads, kv_heads,
-                                         head_dim, num_pages, page_size, max_pages, q_stride, scale,
-                                         int(bool(causal)), _stream(device_idx)), "attention_q4_f32")
-    return o
+    qt, ct, tt, lt, st, ot, wt = q._t, cache._t, page_table._t, kv_lens._t, q_starts._t, out._t, workspace._t
+    if (qt.numel() < nq or ct.numel() < nc or tt.numel() < num_seqs * max_pages * 4 or lt.numel() < num_seqs * 4
+            or st.numel() < ns or ot.numel() < no):
+        _needs("attention", ("q", q, nq), ("cache", cache, nc), ("page_table", page_table, num_seqs * max_pages * 4),
+               ("kv_lens", kv_lens, num_seqs * 4), ("q_starts", q_starts, ns), ("out", out, no))
+    status = lib.kore_hip_attention_q4_f32(
+        qt.data_ptr(), ct.data_ptr(), tt.data_ptr(), lt.data_ptr(), st.data_ptr(), ot.data_ptr(), wt.data_ptr(),
+        wt.numel(), num_seqs, tokens, q_heads, kv_heads, head_dim, num_pages, page_size, max_pages, q_stride, scale,
+        1 if causal else 0, _stream(device_idx))
+    if status:
+        _check(status, "attention_q4_f32")
+    return out
 
 
 __all__ += ["rocm_qk_norm_rope_f32", "rocm_qk_norm_rope_backward_workspace_bytes", "rocm_qk_norm_rope_backward_f32",
