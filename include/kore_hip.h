@@ -407,7 +407,8 @@ uint64_t kore_hip_kv_cache_q4_bytes(uint64_t num_pages, uint64_t page_size,
  * apart, 0: kv_heads * head_dim) go to slot slots[t] = page * page_size + token
  * of the page.  A slot past the last page (0xffffffff of a padded batch) is not
  * written.  Nothing else in the cache changes.  A slot may appear once in a
- * call: if it appears again, what it holds is a mix of its tokens' blocks. */
+ * call: if it appears again, what that slot holds afterwards is a mix of its
+ * tokens' codes and scales. */
 int kore_hip_kv_cache_write_q4_f32(const float *k, const float *v,
                                    const uint32_t *slots, uint8_t *cache,
                                    uint64_t tokens, uint64_t kv_heads,

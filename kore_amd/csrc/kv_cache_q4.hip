@@ -28,7 +28,7 @@ struct Q4Args {
     const uint32_t* slots;
     uint8_t* cache;
     uint64_t stride[2];  // floats between two tokens of k, v
-    uint64_t items;      // tokens * kv_heads * 4 nb
+    uint32_t items;      // tokens * kv_heads * 4 nb
     uint32_t head_dim;
     Q4Cache c;
 };
@@ -40,16 +40,16 @@ __device__ __forceinline__ uint32_t quad_max(uint32_t v) {
 }
 
 // Item i -> token, key head, chunk of eight dimensions.
-__device__ __forceinline__ void q4_item(const Q4Args& a, uint64_t i, uint64_t* token, uint32_t* head, uint32_t* chunk) {
+__device__ __forceinline__ void q4_item(const Q4Args& a, uint32_t i, uint64_t* token, uint32_t* head, uint32_t* chunk) {
     const uint32_t chunks = 4u * a.c.nb, row = chunks * a.c.kv_heads;
     *token = i / row;
-    const uint32_t in_row = (uint32_t)(i - *token * row);
+    const uint32_t in_row = i - (uint32_t)*token * row;
     *head = in_row / chunks;
     *chunk = in_row - *head * chunks;
 }
 
 __global__ __launch_bounds__(kQ4Block) void q4_write_kernel(Q4Args a) {
-    const uint64_t i = (uint64_t)blockIdx.x * kQ4Block + threadIdx.x;
+    const uint32_t i = blockIdx.x * kQ4Block + threadIdx.x;
     const int which = blockIdx.y;  // 0: K, 1: V
     if (i >= a.items) return;      // whole blocks of four lanes leave
     uint64_t token;
@@ -102,7 +102,7 @@ __global__ __launch_bounds__(kQ4Block) void q4_write_kernel(Q4Args a) {
 }
 
 __global__ __launch_bounds__(kQ4Block) void q4_read_kernel(Q4Args a) {
-    const uint64_t i = (uint64_t)blockIdx.x * kQ4Block + threadIdx.x;
+    const uint32_t i = blockIdx.x * kQ4Block + threadIdx.x;
     const int which = blockIdx.y;
     if (i >= a.items) return;
     uint64_t token;
@@ -155,8 +155,8 @@ static int q4_launch(Kernel kernel, Q4Args a, uint64_t tokens, bool write, hipSt
     const uint64_t band = std::max<uint64_t>(1, (1ull << 30) / per_token);
     for (uint64_t t = 0; t < tokens; t += band) {
         const uint64_t n = std::min(band, tokens - t);
-        a.items = n * per_token;
-        hipLaunchKernelGGL(kernel, dim3((uint32_t)((a.items + kQ4Block - 1) / kQ4Block), 2), dim3(kQ4Block), 0, s, a);
+        a.items = (uint32_t)(n * per_token);
+        hipLaunchKernelGGL(kernel, dim3((a.items + kQ4Block - 1) / kQ4Block, 2), dim3(kQ4Block), 0, s, a);
         const int st = launch_status();
         if (st != KORE_HIP_OK) return st;
         a.slots += n;
