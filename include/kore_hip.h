@@ -439,7 +439,7 @@ int kore_hip_kv_cache_read_q4_f32(const uint8_t *cache, const uint32_t *slots,
  * are left out.  Keys and values that a row does not see have no part in it, NaN
  * included.
  * The result is that of the cached values in f32 (f32 tol): products with the
- * 4-bit values are exact, sums f32, probabilities 16 bits.
+ * 4-bit values are exact, scores, probabilities and sums f32.
  * The reference attends in f32 on the CPU (crates/kore-attention/src/flash.rs:28).
  * workspace (16-byte aligned): kore_hip_attention_q4_workspace_bytes bytes,
  * which may be 0; less is KORE_HIP_ERR_BAD_DIM.  Calls that may overlap in time

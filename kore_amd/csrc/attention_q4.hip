@@ -9,10 +9,10 @@
 // gfx950 makes two of them with their scale in one instruction, so the matrix
 // cores' bf16 form loses nothing on the cache's side.  A query value (times scale
 // * log2 e, one f32 rounding) is cut into three bf16 terms of 8 bits each, which
-// is all of its 24: every product q * k is exact and sums are f32.  A probability
-// is two bf16 terms rounded to nearest: it is off by at most 2^-18 of itself, next
-// to the few f32 roundings of the score that it is the exponential of; the row's
-// sum takes the f32 value.
+// is all of its 24: every product q * k is exact and sums are f32.  Probabilities
+// are cut the same way.  With two terms each (2^-18 of a probability lost) results
+// were off by 2.4e-6 of themselves where f32 products are by 6e-7; the third costs
+// a decode step nothing and a prompt a sixth more products.
 // (The block-scaled product takes K's codes and scales as they lie, and q as six
 // E4M3 terms; but its sum keeps only some 2^-19 of the largest product, so blocks
 // of very different scales would cost accuracy that f32 has.)
@@ -44,9 +44,10 @@ constexpr int kAttWaves = kAttBlock / kWave;
 constexpr uint32_t kAttStep = 32;             // tokens of a step
 constexpr uint32_t kAttMinChunk = 8;          // steps of a share, at least
 constexpr uint32_t kAttMaxSteps = 1u << 27;   // more than 2^31 keys have
-constexpr int kAttTerms = 3;                  // bf16 terms of a query value
+constexpr int kAttTerms = 3;                  // bf16 terms of a float
 constexpr uint32_t kAttJoin = 512;            // threads of the joining kernel
 constexpr uint32_t kAttMaxSplits = 1024;
+constexpr uint32_t kAttCus = 256;
 
 struct AttArgs {
     const float* q;
@@ -71,6 +72,7 @@ struct AttItem {
     uint32_t seq, q0, q_len, kv_len;
     uint32_t rows, first;    // rows of the sequence, the tile's first
     uint32_t chunk, split;   // steps of a share, the item's share
+    uint32_t item;           // its number
     uint32_t splits;         // shares of the sequence's keys
     bool ok;
 };
@@ -96,72 +98,98 @@ __device__ __forceinline__ uint32_t att_steps(uint32_t keys) { return (keys + kA
 // Items are numbered through the sequences: a sequence has ceil(len * group /
 // kRows) tiles of ceil(steps / chunk) shares each.  The chunk is the same for all
 // sequences, so that items take equally long however ragged the lengths are: the
-// least (to an eighth) with which there are no more than `target`.  The host
+// least (to an eighth; for more sequences than a wave's lanes hold, to a half) with
+// which there are no more than `target`.  The host
 // knows no lengths; the grid has as many items as there can be, and those past
-// the last are empty.
-template <uint32_t kRows>
-__device__ __forceinline__ AttItem att_item(const AttArgs& a, uint32_t item) {
+// the last are empty.  kTiles: `number` is that of a tile, and its first item is
+// meant.
+template <uint32_t kRows, bool kTiles>
+__device__ __forceinline__ AttItem att_item(const AttArgs& a, uint32_t number) {
+    constexpr int kHeld = 4;  // sequences that a lane holds
     AttItem t = {};
     const uint32_t lim = (uint32_t)a.tokens;
     const uint32_t cap = a.c.num_pages ? a.max_pages << a.c.shift : 0;
-    uint32_t q0 = 0, len = 0, kv = 0;
+    uint32_t q0[kHeld], len[kHeld], kv[kHeld];
     auto read = [&](uint32_t s0) {
-        const uint32_t s = s0 + lane_id();
-        q0 = len = kv = 0;
-        if (s < a.num_seqs) {
-            q0 = min(a.starts[s], lim);
-            const uint32_t q1 = min(a.starts[s + 1], lim);
-            len = q1 > q0 ? q1 - q0 : 0;
-            kv = min(a.lens[s], cap);
+#pragma unroll
+        for (int k = 0; k < kHeld; ++k) {
+            q0[k] = len[k] = kv[k] = 0;
+            const uint32_t s = s0 + k * kWave + lane_id();
+            if (k && s0 + k * kWave >= a.num_seqs) continue;
+            const uint32_t from = a.starts[min(s, a.num_seqs)], to = a.starts[min(s + 1, a.num_seqs)];
+            q0[k] = min(from, lim);
+            len[k] = max(min(to, lim), q0[k]) - q0[k];
+            kv[k] = min(a.lens[min(s, a.num_seqs - 1)], cap);
         }
     };
-    auto tiles = [&] { return (len * a.group + kRows - 1) / kRows; };
-    t.chunk = 0xffffffffu;
+    auto tiles = [&](int k) { return (len[k] * a.group + kRows - 1) / kRows; };
+    const bool one = a.num_seqs <= kHeld * kWave;
+    if (one) read(0);
+    t.chunk = kAttMaxSteps;  // a share a tile
     if (a.target) {
-        // Sum over the sequences of f(tiles, steps).
-        const bool one = a.num_seqs <= kWave;
-        if (one) read(0);
-        auto sum = [&](auto f) {
-            uint64_t all = 0;
-            for (uint32_t s0 = 0; s0 < a.num_seqs; s0 += kWave) {
-                if (!one) read(s0);
-                all += f((uint64_t)tiles(), att_steps(kv));
+        uint64_t all = 0;    // tiles times their steps
+        uint32_t count = 0;  // tiles
+        for (uint32_t s0 = 0; s0 < a.num_seqs; s0 += kHeld * kWave) {
+            if (!one) read(s0);
+            uint64_t n = 0;
+            uint32_t m = 0;
+#pragma unroll
+            for (int k = 0; k < kHeld; ++k) {
+                n += (uint64_t)tiles(k) * att_steps(kv[k]);
+                m += tiles(k);
             }
-            const uint32_t lo = wave_total((uint32_t)all & 0xffffffu), hi = wave_total((uint32_t)(all >> 24));
-            return ((uint64_t)hi << 24) + lo;
-        };
-        const uint64_t all = sum([](uint64_t n, uint32_t steps) { return n * steps; });
-        uint64_t chunk = max((all + a.target - 1) / a.target, (uint64_t)kAttMinChunk);
-        // a chunk of all steps leaves a share a tile
-        while (chunk < kAttMaxSteps && sum([&](uint64_t n, uint32_t steps) {
-                   return n * max((steps + (uint32_t)chunk - 1) / (uint32_t)chunk, 1u);
-               }) > a.target)
-            chunk += (chunk + 7) / 8;
-        t.chunk = (uint32_t)min(chunk, (uint64_t)kAttMaxSteps);
-    }
-    uint32_t before = 0;  // items of the sequences gone by
-    for (uint32_t s0 = 0; s0 < a.num_seqs; s0 += kWave) {
-        if (!a.target || a.num_seqs > kWave) read(s0);  // else it has been
-        const uint32_t splits = a.target ? max((att_steps(kv) + t.chunk - 1) / t.chunk, 1u) : 1u;
-        const uint32_t count = tiles() * splits, sum = wave_scan(count);
-        const uint32_t all = (uint32_t)__builtin_amdgcn_readlane((int)sum, kWave - 1);
-        if (item - before >= all) {
-            before += all;
-            continue;
+            all += ((uint64_t)wave_total((uint32_t)(n >> 24)) << 24) + wave_total((uint32_t)n & 0xffffffu);
+            count += wave_total(m);
         }
-        const int lane = (int)__popcll(__ballot(sum <= item - before));  // sequences that end before the item
-        t.seq = s0 + lane;
-        t.q0 = (uint32_t)__builtin_amdgcn_readlane((int)q0, lane);
-        t.q_len = (uint32_t)__builtin_amdgcn_readlane((int)len, lane);
-        t.kv_len = (uint32_t)__builtin_amdgcn_readlane((int)kv, lane);
-        t.splits = (uint32_t)__builtin_amdgcn_readlane((int)splits, lane);
-        const uint32_t n = (uint32_t)__builtin_amdgcn_readlane((int)count, lane);
-        const uint32_t at = item - before - ((uint32_t)__builtin_amdgcn_readlane((int)sum, lane) - n);
-        t.rows = t.q_len * a.group;
-        t.split = at % t.splits;
-        t.first = (n / t.splits - 1 - at / t.splits) * kRows;  // the rows that see the most keys first
-        t.ok = true;
-        return t;
+        // n tiles in shares of c steps make fewer than all / c + n: the chunk lies
+        // between all / target and all / (target - n).
+        if (count < a.target) {
+            const uint64_t most = (all + a.target - count - 1) / (a.target - count);
+            uint64_t chunk = max(one ? (all + a.target - 1) / a.target : most, (uint64_t)kAttMinChunk);
+            while (chunk < most) {  // the sequences are in registers
+                uint64_t n = 0;     // shares
+#pragma unroll
+                for (int k = 0; k < kHeld; ++k)
+                    if (k == 0 || k * kWave < (int)a.num_seqs)
+                        n += (uint64_t)tiles(k) * max((att_steps(kv[k]) + (uint32_t)chunk - 1) / (uint32_t)chunk, 1u);
+                if (wave_total((uint32_t)min(n, (uint64_t)1 << 25)) <= a.target) break;
+                chunk += (chunk + 7) / 8;
+            }
+            t.chunk = (uint32_t)min(chunk, (uint64_t)kAttMaxSteps);
+        }
+    }
+    uint32_t before = 0, items = 0;  // numbers, items of the sequences gone by
+    for (uint32_t s0 = 0; s0 < a.num_seqs; s0 += kHeld * kWave) {
+        if (!one) read(s0);
+#pragma unroll
+        for (int k = 0; k < kHeld; ++k) {
+            if (k && s0 + k * kWave >= a.num_seqs) break;
+            const uint32_t splits = max((att_steps(kv[k]) + t.chunk - 1) / t.chunk, 1u);
+            const uint32_t n = tiles(k), count = kTiles ? n : n * splits, sum = wave_scan(count);
+            const uint32_t sum_items = kTiles ? wave_scan(n * splits) : sum;
+            const uint32_t all = (uint32_t)__builtin_amdgcn_readlane((int)sum, kWave - 1);
+            if (number - before >= all) {
+                before += all;
+                items += (uint32_t)__builtin_amdgcn_readlane((int)sum_items, kWave - 1);
+                continue;
+            }
+            // sequences that end before it
+            const int lane = (int)__popcll(__ballot(sum <= number - before));
+            auto of = [&](uint32_t v) { return (uint32_t)__builtin_amdgcn_readlane((int)v, lane); };
+            t.seq = s0 + k * kWave + lane;
+            t.q0 = of(q0[k]);
+            t.q_len = of(len[k]);
+            t.kv_len = of(kv[k]);
+            t.splits = of(splits);
+            const uint32_t mine = of(n), at = number - before - (of(sum) - of(count));
+            const uint32_t tile = kTiles ? at : at / t.splits;
+            t.split = kTiles ? 0 : at % t.splits;
+            t.item = kTiles ? items + of(sum_items) - (mine - tile) * t.splits : number;
+            t.rows = t.q_len * a.group;
+            t.first = (mine - 1 - tile) * kRows;  // the rows that see the most keys first
+            t.ok = true;
+            return t;
+        }
     }
     return t;
 }
@@ -203,13 +231,13 @@ __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
                                                    0, 0);
 }
 
-// Two floats as bf16 (to nearest) in one register, and what that left over.
-__device__ __forceinline__ uint32_t pack_bf16(float x, float y, float* rx, float* ry) {
-    const bf16x2 v = {(__bf16)x, (__bf16)y};
-    const uint32_t u = __builtin_bit_cast(uint32_t, v);
-    *rx = x - __uint_as_float(u << 16);
-    *ry = y - __uint_as_float(u & 0xffff0000u);
-    return u;
+// The top 16 bits (a bf16) of two floats.
+__device__ __forceinline__ uint32_t pack_top(float x, float y) {
+    return perm(__float_as_uint(y), __float_as_uint(x), 0x07060302u);
+}
+// What the bf16 that `mask` keeps of x leaves over.
+__device__ __forceinline__ float rest(float x, uint32_t mask = 0xffff0000u) {
+    return x - __uint_as_float(__float_as_uint(x) & mask);
 }
 
 // Row r's query.
@@ -239,10 +267,9 @@ __device__ __forceinline__ void query_terms(const AttArgs& a, const float* q, ui
         float u = x[2 * i] * a.scale_log2, v = x[2 * i + 1] * a.scale_log2;
 #pragma unroll
         for (int k = 0; k < kAttTerms; ++k) {
-            const uint32_t ub = __float_as_uint(u), vb = __float_as_uint(v);
-            term[k][i] = perm(vb, ub, 0x07060302u);
-            u -= __uint_as_float(ub & 0xffff0000u);
-            v -= __uint_as_float(vb & 0xffff0000u);
+            term[k][i] = pack_top(u, v);
+            u = rest(u);
+            v = rest(v);
         }
     }
 }
@@ -381,10 +408,9 @@ struct AttKV {
 
 // NB: blocks of 32 dimensions that the tiles hold (2, 4 or 8), nb <= NB of them
 // in use.  kSlot: rows of a matrix tile's 16 columns.  16: a product for each of
-// q's three terms and each of p's two.  With 8 or 4 rows (a decode step's query
-// heads) the terms lie side by side in the columns instead, column = slot * kSlot +
-// row: one product takes two or all three of q's terms and both of p's, and the
-// slots' scores are added across lanes.
+// three terms of q, and of p.  With 8 or 4 rows (a decode step's query heads) the
+// terms lie side by side in the columns instead, column = slot * kSlot + row: one
+// product takes two or all three, and the slots' scores are added across lanes.
 // R: 16-row tiles of a wave.  An item's rows are kSlot, or with R = 2 four waves'
 // 128: the waves deal out the rows, and where there are too few rows for four
 // waves, the tokens, whose parts they join at the end.
@@ -394,7 +420,7 @@ struct AttShape {
     static constexpr uint32_t kRows = kSlot < 16 ? kSlot : 16 * R * kAttWaves;
     static constexpr int kSide = 16 / kSlot;                       // terms side by side
     static constexpr int kQ = (kAttTerms + kSide - 1) / kSide;     // products for a score
-    static constexpr int kP = kSlot == 16 ? 2 : 1;                 // products for an output
+    static constexpr int kP = kQ;                                  // products for an output
 };
 
 // A step, v_mfma_f32_16x16x32_bf16: for S^T a lane holds token n's dimensions of
@@ -413,7 +439,7 @@ void att_kernel(AttArgs a) {
     // Key heads change fastest: workgroups go round the 8 XCDs, and every XCD gets
     // its part of the items, of which the last may be empty.
     const uint32_t head = blockIdx.x % a.c.kv_heads, item = a.item0 + blockIdx.x / a.c.kv_heads;
-    const AttItem t = att_item<kRows>(a, item);
+    const AttItem t = att_item<kRows, false>(a, item);
     if (!t.ok) return;
     const uint32_t nb = a.c.nb;
     // The item's share of its steps: [lo, hi).
@@ -430,9 +456,26 @@ void att_kernel(AttArgs a) {
     const uint32_t min_limit = att_limit(a, t, min(r0, t.rows - 1));
     const uint32_t end = r0 < r1 ? min(hi, att_steps(att_limit(a, t, r1 - 1))) : 0;
 
+    // Products before other waves' softmax: 8192 x 45, 8 key heads of 128, 4 query
+    // heads each 52.3 -> 50.9 us, 8 each (64 sequences) 78 -> 73; with 16-row columns
+    // 16 rows a sequence lost (65 -> 71 us) what long chunks gained (106 -> 99).
+    constexpr bool kRaise = kSlot < 16 && NB < 8;
+    // q's third term lies in LDS where the registers would not hold it (4 x 4096
+    // tokens, 32 + 8 heads of 128: 1295 -> 1193 us, the spills gone).
+    constexpr bool kPark = kSlot == 16 && R == 2 && NB == 4;
+    constexpr int kHeldQ = kPark ? kQ - 1 : kQ;
+    union Shared {
+        float so[kAttWaves][16][16 * kJ + 4];
+        u32x4 q[kPark ? kAttWaves : 1][R][NB][kWave];
+        __device__ Shared() {}
+    };
+    __shared__ __attribute__((aligned(16))) Shared shared;
     const uint32_t slot = n / kSlot;
+    // What a lane of slot 1, and of slot 2, leaves out of a probability before its own term.
+    const uint32_t cut1 = kSlot < 16 && slot >= 1 ? 0xffff0000u : 0, cut2 = kSlot < 16 && slot >= 2 ? 0xffff0000u : 0;
+    const uint32_t slot1 = slot ? 0xffffffffu : 0;
     uint32_t limit[R];
-    u32x4 qf[R][kQ][NB];
+    u32x4 qf[R][kHeldQ][NB];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
         const uint32_t row = r0 + 16 * r + n % kSlot;
@@ -449,7 +492,8 @@ void att_kernel(AttArgs a) {
 #pragma unroll
                 for (int at = 0; at < kSide; ++at)
                     if (k * kSide + at < kAttTerms && slot == (uint32_t)at) w = term[k * kSide + at];
-                qf[r][k][j] = w;
+                if (k < kHeldQ) qf[r][k][j] = w;
+                else shared.q[wave][r][j][lane] = w;
             }
         }
     }
@@ -504,20 +548,26 @@ void att_kernel(AttArgs a) {
     };
 
     auto work = [&](uint32_t step, AttKV<NB> (&cur)[2], const uint32_t (&page)[2]) {
+        if constexpr (kRaise) __builtin_amdgcn_s_setprio(1);
         // Scores, in powers of two: tokens 4g + i of both tiles.
         f32x4 s[R][2];
 #pragma unroll
         for (int r = 0; r < R; ++r) s[r][0] = s[r][1] = zero;
 #pragma unroll
-        for (int j = 0; j < NB; ++j)
+        for (int j = 0; j < NB; ++j) {
+            u32x4 q3[R];
+            if constexpr (kPark)
+#pragma unroll
+                for (int r = 0; r < R; ++r) q3[r] = shared.q[wave][r][j][lane];
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
                 const u32x4 kf = cvt8(cur[x].k[j], byte_scale(cur[x].ks[j / 4], 0));
 #pragma unroll
                 for (int k = kQ - 1; k >= 0; --k)
 #pragma unroll
-                    for (int r = 0; r < R; ++r) s[r][x] = mfma(kf, qf[r][k][j], s[r][x]);
+                    for (int r = 0; r < R; ++r) s[r][x] = mfma(kf, k < kHeldQ ? qf[r][k < kHeldQ ? k : 0][j] : q3[r], s[r][x]);
             }
+        }
         if constexpr (kSlot < 16) {
 #pragma unroll
             for (int x = 0; x < 2; ++x)
@@ -544,6 +594,7 @@ void att_kernel(AttArgs a) {
                 cur[x].vs = finite_scales(cur[x].vs, 4 * g, cur[x].valid, &nan_v);
             }
         }
+        if constexpr (kRaise) __builtin_amdgcn_s_setprio(0);
         // Running maximum, probabilities and their sum; bf16 terms.
         u32x4 pf[R][kP];
 #pragma unroll
@@ -565,16 +616,19 @@ void att_kernel(AttArgs a) {
                     const float p0 = __builtin_amdgcn_exp2f(s[r][x][i] - top[r].base);
                     const float p1 = __builtin_amdgcn_exp2f(s[r][x][i + 1] - top[r].base);
                     l[r] += p0 + p1;
-                    float e0, e1, u0, u1;
-                    const uint32_t first = pack_bf16(p0, p1, &e0, &e1);
-                    if constexpr (kSlot == 16) {
-                        pf[r][0][2 * x + i / 2] = first;
-                        pf[r][1][2 * x + i / 2] = pack_bf16(e0, e1, &u0, &u1);
-                    } else {  // slot 0 holds the first term, slot 1 the second; the others are not read
-                        pf[r][0][2 * x + i / 2] = slot ? pack_bf16(e0, e1, &u0, &u1) : first;
+                    // the lane's term (slot 3's column is not read)
+                    float u0 = rest(p0, cut1), u1 = rest(p1, cut1);
+                    if constexpr (kSlot == 4) u0 = rest(u0, cut2), u1 = rest(u1, cut2);
+#pragma unroll
+                    for (int k = 0; k < kP; ++k) {
+                        pf[r][k][2 * x + i / 2] = pack_top(u0, u1);
+                        u0 = rest(u0);
+                        u1 = rest(u1);
                     }
+                    if constexpr (kSlot == 8) pf[r][1][2 * x + i / 2] &= slot1;  // the third term is slot 1's
                 }
         }
+        if constexpr (kRaise) __builtin_amdgcn_s_setprio(1);
         // V: four dwords a tile are four tokens x eight dimensions; an operand is
         // eight tokens of one dimension.
         float vsc[8];
@@ -600,6 +654,7 @@ void att_kernel(AttArgs a) {
                     for (int r = 0; r < R; ++r) o[r][2 * p + h] = mfma(vf, pf[r][k], o[r][2 * p + h]);
             }
         }
+        if constexpr (kRaise) __builtin_amdgcn_s_setprio(0);
         if (!whole && __any(nan_v)) {
 #pragma unroll
             for (int x = 0; x < 2; ++x)
@@ -671,7 +726,7 @@ void att_kernel(AttArgs a) {
     // Join the waves of a group: to the common maximum, then add (and the second
     // term's column to the first's).
     __shared__ float sm[kAttWaves][16], sl[kAttWaves][16];
-    __shared__ __attribute__((aligned(16))) float so[kAttWaves][16][16 * kJ + 4];
+    auto& so = shared.so;
 #pragma unroll
     for (int r = 0; r < R; ++r) {
         __syncthreads();
@@ -699,7 +754,9 @@ void att_kernel(AttArgs a) {
                 const float f = sm[w][row] == ninf ? 1.0f : __builtin_amdgcn_exp2f(sm[w][row] - mm);
                 ll += sl[w][row] * f;
                 f32x4 u = *reinterpret_cast<const f32x4*>(&so[w][row][d]);
-                if (kSlot < 16) u += *reinterpret_cast<const f32x4*>(&so[w][row + kSlot % 16][d]);
+#pragma unroll
+                for (int at = 1; at < kSide && at < kAttTerms; ++at)
+                    u += *reinterpret_cast<const f32x4*>(&so[w][row + at * kSlot][d]);
 #pragma unroll
                 for (int k = 0; k < 4; ++k) v[k] += u[k] * f;
             }
@@ -708,60 +765,102 @@ void att_kernel(AttArgs a) {
     }
 }
 
-// Joins the shares of a tile, kJoinRows rows at a time: their maxima and sums
-// through LDS, then a thread has four dimensions of a row and every kth share.
-constexpr uint32_t kJoinRows = 4;
+// Joins the shares of a tile.  Few shares: a thread has four dimensions of a row and
+// all shares, in flight together.  Many: kJoinRows rows at a time, their maxima and
+// sums through LDS, and a thread has four dimensions of a row and every kth share.
+constexpr uint32_t kJoinRows = 4, kJoinFew = 8;
+
+template <uint32_t kRows>
+struct AttJoin {
+    static constexpr uint32_t kParts = kRows <= 32 ? 1 : kRows / 32;  // workgroups of a tile
+};
+
+// Four dimensions of row rr, their sum l.
+__device__ __forceinline__ void join_store(const AttArgs& a, const AttItem& t, uint32_t head, uint32_t rr, uint32_t d,
+                                           float l, f32x4 v) {
+    float* out = a.out + ((uint64_t)(t.q0 + rr / a.group) * a.q_heads + head * a.group + rr % a.group) * a.dim + d;
+    const float f = 1.0f / l;
+    f32x4 u;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) u[k] = l == 0.0f ? 0.0f : v[k] * f;
+    if (d + 4 <= a.dim) {
+        *reinterpret_cast<f32x4_a4*>(out) = (f32x4_a4)u;
+    } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (d + k < a.dim) out[k] = u[k];
+    }
+}
 
 template <uint32_t kRows>
 __global__ __launch_bounds__(kAttJoin) void att_join_kernel(AttArgs a) {
+    constexpr uint32_t kParts = AttJoin<kRows>::kParts, kPart = kRows / kParts;
     __shared__ float2 ml[kJoinRows][kAttMaxSplits];
     __shared__ f32x4 red[kAttJoin];
-    const uint32_t head = blockIdx.x % a.c.kv_heads, item = a.item0 + blockIdx.x / a.c.kv_heads;
-    const AttItem t = att_item<kRows>(a, item);
-    if (!t.ok || t.split || t.splits == 1) return;
+    const uint32_t tile = blockIdx.x / kParts, from = blockIdx.x % kParts * kPart, head = tile % a.c.kv_heads;
+    const AttItem t = att_item<kRows, true>(a, tile / a.c.kv_heads);
+    if (!t.ok || t.splits == 1 || t.first + from >= t.rows) return;
+    const uint32_t count = min(kPart, t.rows - t.first - from);  // rows of this workgroup
     const uint32_t last_row = min(t.first + kRows, t.rows) - 1;
     const uint32_t used = (att_steps(att_limit(a, t, last_row)) + t.chunk - 1) / t.chunk;
     const uint64_t next = (uint64_t)a.c.kv_heads * kRows;  // rows to the next share's
-    const float* po = a.part + (uint64_t)a.items * a.c.kv_heads * kRows * 2;
-    const uint32_t dp = 32 * a.c.nb, quads = dp / 4, group = kJoinRows * quads, groups = kAttJoin / group;
-    const uint32_t gr = threadIdx.x / group, row = threadIdx.x % group / quads, d = threadIdx.x % quads * 4;
-    for (uint32_t row0 = 0; row0 < kRows && t.first + row0 < t.rows; row0 += kJoinRows) {
-        const uint64_t part0 = ((uint64_t)item * a.c.kv_heads + head) * kRows + row0;
-        const float2* pm = reinterpret_cast<const float2*>(a.part) + part0;
+    const uint32_t dp = 32 * a.c.nb, quads = dp / 4, d = threadIdx.x % quads * 4;
+    const uint64_t part0 = ((uint64_t)t.item * a.c.kv_heads + head) * kRows + from;
+    const float2* pm = reinterpret_cast<const float2*>(a.part) + part0;
+    const float* po = a.part + (uint64_t)a.items * a.c.kv_heads * kRows * 2 + part0 * dp + d;
+    const float ninf = -__builtin_inff();
+    // What a share's sum and outputs are multiplied by: one that saw nothing holds
+    // zeros (or NaN, which stays).
+    auto factor = [&](float m, float mm) { return m == ninf ? 1.0f : __builtin_amdgcn_exp2f(m - mm); };
+    if (used <= kJoinFew) {
+        for (uint32_t row = threadIdx.x / quads; row < count; row += kAttJoin / quads) {
+            if (threadIdx.x >= kAttJoin / quads * quads) break;  // lanes past the last whole row
+            float2 u[kJoinFew];
+            f32x4 w[kJoinFew];
+#pragma unroll
+            for (uint32_t z = 0; z < kJoinFew; ++z) {
+                const uint32_t at = z < used ? z : 0;
+                u[z] = pm[at * next + row];
+                w[z] = *reinterpret_cast<const f32x4*>(po + (at * next + row) * dp);
+            }
+            float mm = ninf, ll = 0.0f;
+            f32x4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (uint32_t z = 0; z < kJoinFew; ++z) mm = fmaxf(mm, u[z].x);
+#pragma unroll
+            for (uint32_t z = 0; z < kJoinFew; ++z)
+                if (z < used) {
+                    const float f = factor(u[z].x, mm);
+                    ll += u[z].y * f;
+                    v += w[z] * f;
+                }
+            join_store(a, t, head, t.first + from + row, d, ll, v);
+        }
+        return;
+    }
+    const uint32_t group = kJoinRows * quads, groups = kAttJoin / group;
+    const uint32_t gr = threadIdx.x / group, row = threadIdx.x % group / quads;
+    for (uint32_t row0 = 0; row0 < count; row0 += kJoinRows) {
         __syncthreads();
         // rows past the sequence's hold anything and are not stored
         for (uint32_t i = threadIdx.x; i < used * kJoinRows; i += kAttJoin)
-            ml[i % kJoinRows][i / kJoinRows] = pm[i / kJoinRows * next + i % kJoinRows];
+            ml[i % kJoinRows][i / kJoinRows] = pm[i / kJoinRows * next + row0 + i % kJoinRows];
         __syncthreads();
-        const float ninf = -__builtin_inff();
         float mm = ninf, ll = 0.0f;
         f32x4 v = {0.f, 0.f, 0.f, 0.f};
         if (gr < groups) {
             for (uint32_t z = 0; z < used; ++z) mm = fmaxf(mm, ml[row][z].x);
-            const float* p = po + (part0 + row) * dp + d;
+            const float* p = po + (uint64_t)(row0 + row) * dp;
 #pragma unroll 8
-            for (uint32_t z = gr; z < used; z += groups) {
-                const float2 u = ml[row][z];
-                // a share that saw nothing holds zeros (or NaN, which stays)
-                const float f = u.x == ninf ? 1.0f : __builtin_amdgcn_exp2f(u.x - mm);
-                v += *reinterpret_cast<const f32x4*>(p + z * next * dp) * f;
-            }
+            for (uint32_t z = gr; z < used; z += groups)
+                v += *reinterpret_cast<const f32x4*>(p + z * next * dp) * factor(ml[row][z].x, mm);
         }
         red[threadIdx.x] = v;
         __syncthreads();
-        const uint32_t rr = t.first + row0 + row;
-        if (gr == 0 && rr < t.rows) {
-            for (uint32_t k = 1; k < groups; ++k) v += red[threadIdx.x + k * group];
-            for (uint32_t z = 0; z < used; ++z) {
-                const float2 u = ml[row][z];
-                ll += u.x == ninf ? u.y : u.y * __builtin_amdgcn_exp2f(u.x - mm);
-            }
-            float* out = a.out + ((uint64_t)(t.q0 + rr / a.group) * a.q_heads + head * a.group + rr % a.group) * a.dim;
-            const float f = 1.0f / ll;
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-                if (d + k < a.dim) out[d + k] = ll == 0.0f ? 0.0f : v[k] * f;
-        }
+        if (gr != 0 || row0 + row >= count) continue;
+        for (uint32_t k = 1; k < groups; ++k) v += red[threadIdx.x + k * group];
+        for (uint32_t z = 0; z < used; ++z) ll += ml[row][z].y * factor(ml[row][z].x, mm);
+        join_store(a, t, head, t.first + from + row0 + row, d, ll, v);
     }
 }
 
@@ -769,22 +868,40 @@ __global__ __launch_bounds__(kAttJoin) void att_join_kernel(AttArgs a) {
 // four waves.
 struct AttPlan {
     uint32_t rows;  // kRows: 4, 8 (kSlot), 64 or 128 (kSlot 16)
-    uint32_t items, target;
+    uint32_t tiles, items, target;
     uint64_t bytes;  // workspace
 };
 
+// Sizes decide what the device cannot wait to see; lengths are not known here.
+//
+// Rows.  Prompts whose 128-row items fit on the chip all at once (two workgroups a
+// CU) take 64-row items: they end evenly (2048 tokens, 32 + 8 heads of 128: 105 ->
+// 85 us; 512 tokens 30 -> 18).  With more, 128 rows need a key's and a value's
+// conversion half as often (4 x 4096 of 16 heads of 64: 152 us, with 64 rows 160).
+//
+// Cut.  Keys are cut where the tiles are fewer than the workgroups that the chip
+// holds at once.  45 decode steps over up to 8192 tokens, 8 key heads: 67 -> 53 us;
+// 96 of them: 108 us, cut 114; 4 x 256 tokens after 32768: 1031 -> 608 us.  Below
+// 2048 tokens the second kernel costs more than the shares save (1 x 1024: 10.4 us,
+// cut 12.1; 1 x 2048: 12.0 us, uncut 15.8).
 static int att_plan(uint64_t num_seqs, uint64_t tokens, uint64_t q_heads, uint64_t kv_heads, uint64_t page_size,
                     uint64_t max_pages, uint32_t nb, AttPlan* p) {
     const uint64_t group = q_heads / kv_heads, rows = tokens * group;
-    p->rows = rows <= 4 * num_seqs ? 4 : rows <= 8 * num_seqs ? 8 : rows <= 16 * num_seqs || nb > 4 ? 64 : 128;
-    const uint64_t tiles = rows / p->rows + num_seqs;
+    p->rows = rows <= 4 * num_seqs                                                       ? 4
+              : rows <= 8 * num_seqs                                                     ? 8
+              : rows <= 16 * num_seqs || nb > 4 || rows / 128 * kv_heads <= 2 * kAttCus ? 64
+                                                                                         : 128;
+    const uint64_t some = std::min(num_seqs, tokens);  // sequences with new tokens, at most
+    const uint64_t tiles = rows / p->rows + some;
     if (tiles > 0x3fffffull) return KORE_HIP_ERR_OVERFLOW;
-    // Workgroups that the keys are cut for: what the chip holds at once.
-    const uint64_t want = p->rows == 4 && nb <= 4 ? 768 : 512;
-    const uint64_t busy = std::max(std::min(num_seqs, tokens), rows / p->rows) * kv_heads;
+    const uint64_t want = (p->rows == 4 && nb <= 4 ? 3 : 2) * kAttCus;  // workgroups that the chip holds at once
+    const uint64_t busy = std::max(some, rows / p->rows);
     const uint64_t shares = max_pages * page_size / (kAttMinChunk * kAttStep);  // of the longest sequence
-    const bool cut = busy < (rows <= 16 * num_seqs ? 2 * want : want / 2) && shares > 1;
-    p->target = cut ? (uint32_t)std::min<uint64_t>({(want + kv_heads - 1) / kv_heads, tiles * shares, kAttMaxSplits}) : 0;
+    const bool cut = busy * kv_heads < want && shares >= 8;
+    p->target = cut ? (uint32_t)std::min<uint64_t>({std::max((want + kv_heads - 1) / kv_heads, 2 * busy),
+                                                    tiles * shares, kAttMaxSplits})
+                    : 0;
+    p->tiles = (uint32_t)tiles;
     p->items = std::max((uint32_t)tiles, p->target);
     p->bytes = cut ? (uint64_t)p->items * kv_heads * p->rows * (2 + 32ull * nb) * 4 : 0;
     return KORE_HIP_OK;
@@ -803,21 +920,25 @@ static int att_check(uint64_t num_seqs, uint64_t tokens, uint64_t q_heads, uint6
     return att_plan(num_seqs, tokens, q_heads, kv_heads, page_size, max_pages, c->nb, p);
 }
 
+// join: the tiles whose shares are joined, or 0 for the items' kernel.
 template <int NB, int R, int kSlot, int kPerSimd>
-static void att_launch_shape(const AttArgs& a, bool join, dim3 grid, hipStream_t s) {
-    if (join)
-        hipLaunchKernelGGL((att_join_kernel<AttShape<NB, R, kSlot>::kRows>), grid, dim3(kAttJoin), 0, s, a);
-    else
+static void att_launch_shape(const AttArgs& a, uint32_t join, dim3 grid, hipStream_t s) {
+    constexpr uint32_t kRows = AttShape<NB, R, kSlot>::kRows;
+    if (join) {
+        grid = dim3(join * a.c.kv_heads * AttJoin<kRows>::kParts);
+        hipLaunchKernelGGL((att_join_kernel<kRows>), grid, dim3(kAttJoin), 0, s, a);
+    } else {
         hipLaunchKernelGGL((att_kernel<NB, R, kSlot, kPerSimd>), grid, dim3(kAttBlock), 0, s, a);
+    }
 }
 
 // kPerSimd: the waves that a SIMD's registers hold.
-static void att_launch(const AttArgs& a, uint32_t rows, bool join, dim3 grid, hipStream_t s) {
+static void att_launch(const AttArgs& a, uint32_t rows, uint32_t join, dim3 grid, hipStream_t s) {
     auto launch = [&](auto blocks) {
         constexpr int NB = decltype(blocks)::value;
         if (rows == 4) att_launch_shape<NB, 1, 4, NB == 8 ? 2 : 3>(a, join, grid, s);
-        else if (rows == 8) att_launch_shape<NB, 1, 8, NB == 8 ? 1 : 2>(a, join, grid, s);
-        else if (rows == 64) att_launch_shape<NB, 1, 16, NB == 8 ? 1 : 2>(a, join, grid, s);
+        else if (rows == 8) att_launch_shape<NB, 1, 8, NB == 8 ? 1 : NB == 4 ? 3 : 4>(a, join, grid, s);
+        else if (rows == 64) att_launch_shape<NB, 1, 16, NB == 8 ? 1 : NB == 4 ? 2 : 3>(a, join, grid, s);
         else if constexpr (NB < 8) att_launch_shape<NB, 2, 16, 2>(a, join, grid, s);
     };
     if (a.c.nb <= 2) launch(std::integral_constant<int, 2>());
@@ -892,13 +1013,14 @@ extern "C" int kore_hip_attention_q4_f32(const float* q, const uint8_t* cache, c
     a.causal = causal != 0;
     // A launch holds fewer than 2^32 threads: items in bands.
     const uint32_t band = (uint32_t)std::max<uint64_t>(1, 0x400000u / kv_heads);
-    for (int join = 0; join < (p.target ? 2 : 1); ++join) {
-        for (a.item0 = 0; a.item0 < p.items; a.item0 += band) {
-            const uint32_t x = std::min(band, p.items - a.item0) * (uint32_t)kv_heads;
-            att_launch(a, p.rows, join != 0, dim3(x), (hipStream_t)stream);
-            const int rc = launch_status();
-            if (rc != KORE_HIP_OK) return rc;
-        }
+    for (a.item0 = 0; a.item0 < p.items; a.item0 += band) {
+        att_launch(a, p.rows, 0, dim3(std::min(band, p.items - a.item0) * (uint32_t)kv_heads), (hipStream_t)stream);
+        const int rc = launch_status();
+        if (rc != KORE_HIP_OK) return rc;
+    }
+    if (p.target) {  // few tiles, or their keys would not be cut
+        att_launch(a, p.rows, p.tiles, dim3(), (hipStream_t)stream);
+        return launch_status();
     }
     return KORE_HIP_OK;
 }

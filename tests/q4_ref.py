@@ -95,8 +95,8 @@ def attention(q, cache: Cache, table, lens, starts, scale, causal, out):
 
     Off by: a score's error is `u` for q's rounding, and for the sum of 3 nb products of 32 terms at most 3 * 8 + 8 roundings,
     all relative to scale * sum |q k|; the subtraction of the maximum and the exponential 2 u of the score's size and 2 u.
-    A probability has half a step of two bf16 terms, 2^-18, on top; the row's sums add a rounding for each step of 32
-    keys, 64 for joining what was split, and the division."""
+    A probability's three bf16 terms are all of its bits; the row's sums add three roundings for each step of 32 keys
+    (a product for each term), 64 for joining what was split, and the division."""
     tokens, q_heads, d = q.shape
     heads = cache.bytes.shape[1]
     group = q_heads // heads
@@ -126,7 +126,7 @@ def attention(q, cache: Cache, table, lens, starts, scale, causal, out):
                     o[i, h] = p @ vv
                     size = np.abs(kk) @ np.abs(qq) * abs(scale)
                     delta = 33 * U * size.max() + 2 * U * np.abs(x).max() + 2 * U
-                    tol[i, h] = p @ np.abs(vv) * (2.0 ** -18 + 2 * delta + (len(seen) / 32 + 64) * U)
+                    tol[i, h] = p @ np.abs(vv) * (2 * delta + (3 * len(seen) / 32 + 64) * U)
     return o, tol
 
 

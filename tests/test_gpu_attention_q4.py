@@ -77,11 +77,14 @@ def test_against_64_bits(case, causal):
 
 @pytest.mark.parametrize("hq,hk,d,page,lens,news", [(4, 1, 128, 16, [3000], [1]), (8, 2, 64, 64, [5000, 1500], [1, 1]),
                                                     (2, 2, 256, 16, [1200, 0, 40], [2, 1, 1]), (4, 2, 128, 32, [2100], [9]),
-                                                    (6, 1, 96, 16, [1700, 300], [40, 2])])
+                                                    (6, 1, 96, 16, [1700, 300], [40, 2]), (2, 2, 256, 16, [2300, 0, 40], [2, 1, 1]),
+                                                    (6, 1, 96, 16, [3100, 300], [40, 2]), (4, 1, 128, 64, [4097, 700, 2048], [100, 3, 33]),
+                                                    (2, 1, 64, 16, [2500] + [30] * 300, [1] * 301)])
 def test_split_contexts(hq, hk, d, page, lens, news):
     """Few rows over many keys: shares of the keys, joined at the end; some shares of the shorter sequences are empty."""
     c = Case(hq, hk, d, page, lens, news, seed=3, std=3.0)
-    assert rocm.rocm_attention_q4_workspace_bytes(len(lens), c.tokens, hq, hk, d, page, c.most) > 0
+    # keys are cut where the table has room for 2048 tokens of a sequence
+    assert (rocm.rocm_attention_q4_workspace_bytes(len(lens), c.tokens, hq, hk, d, page, c.most) > 0) == (max(lens) >= 2048)
     c.check()
     c.check(causal=False)
 
