@@ -45,7 +45,6 @@ constexpr uint32_t kAttStep = 32;             // tokens of a step
 constexpr uint32_t kAttMinChunk = 8;          // steps of a share, at least
 constexpr uint32_t kAttMaxSteps = 1u << 27;   // more than 2^31 keys have
 constexpr int kAttTerms = 3;                  // bf16 terms of a float
-constexpr uint32_t kAttJoin = 512;            // threads of the joining kernel
 constexpr uint32_t kAttMaxSplits = 1024;
 constexpr uint32_t kAttCus = 256;
 
@@ -765,16 +764,6 @@ void att_kernel(AttArgs a) {
     }
 }
 
-// Joins the shares of a tile.  Few shares: a thread has four dimensions of a row and
-// all shares, in flight together.  Many: kJoinRows rows at a time, their maxima and
-// sums through LDS, and a thread has four dimensions of a row and every kth share.
-constexpr uint32_t kJoinRows = 4, kJoinFew = 8;
-
-template <uint32_t kRows>
-struct AttJoin {
-    static constexpr uint32_t kParts = kRows <= 32 ? 1 : kRows / 32;  // workgroups of a tile
-};
-
 // Four dimensions of row rr, their sum l.
 __device__ __forceinline__ void join_store(const AttArgs& a, const AttItem& t, uint32_t head, uint32_t rr, uint32_t d,
                                            float l, f32x4 v) {
@@ -792,76 +781,140 @@ __device__ __forceinline__ void join_store(const AttArgs& a, const AttItem& t, u
     }
 }
 
-template <uint32_t kRows>
-__global__ __launch_bounds__(kAttJoin) void att_join_kernel(AttArgs a) {
-    constexpr uint32_t kParts = AttJoin<kRows>::kParts, kPart = kRows / kParts;
-    __shared__ float2 ml[kJoinRows][kAttMaxSplits];
-    __shared__ f32x4 red[kAttJoin];
-    const uint32_t tile = blockIdx.x / kParts, from = blockIdx.x % kParts * kPart, head = tile % a.c.kv_heads;
-    const AttItem t = att_item<kRows, true>(a, tile / a.c.kv_heads);
-    if (!t.ok || t.splits == 1 || t.first + from >= t.rows) return;
-    const uint32_t count = min(kPart, t.rows - t.first - from);  // rows of this workgroup
+// What a share's sum and outputs are multiplied by, its maximum m, all shares' mm:
+// one that saw nothing holds zeros (or NaN, which stays).
+__device__ __forceinline__ float join_factor(float m, float mm) {
+    return m == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(m - mm);
+}
+
+// The shares of `count` rows of a tile from row `from` on.
+struct JoinRows {
+    AttItem t;
+    uint32_t head, from, count, used, dp;
+    uint64_t next;     // rows to the next share's
+    const float2* ml;  // maximum and sum of the first row in the first share
+    const float* out;  // its outputs
+};
+
+template <uint32_t kRows, uint32_t kParts>
+__device__ __forceinline__ JoinRows join_rows(const AttArgs& a) {
+    JoinRows j;
+    const uint32_t tile = blockIdx.x / kParts;
+    j.from = blockIdx.x % kParts * (kRows / kParts);
+    j.head = tile % a.c.kv_heads;
+    j.t = att_item<kRows, true>(a, tile / a.c.kv_heads);
+    const AttItem& t = j.t;
+    j.count = !t.ok || t.splits == 1 || t.first + j.from >= t.rows ? 0 : min(kRows / kParts, t.rows - t.first - j.from);
+    if (j.count == 0) return j;
     const uint32_t last_row = min(t.first + kRows, t.rows) - 1;
-    const uint32_t used = (att_steps(att_limit(a, t, last_row)) + t.chunk - 1) / t.chunk;
-    const uint64_t next = (uint64_t)a.c.kv_heads * kRows;  // rows to the next share's
-    const uint32_t dp = 32 * a.c.nb, quads = dp / 4, d = threadIdx.x % quads * 4;
-    const uint64_t part0 = ((uint64_t)t.item * a.c.kv_heads + head) * kRows + from;
-    const float2* pm = reinterpret_cast<const float2*>(a.part) + part0;
-    const float* po = a.part + (uint64_t)a.items * a.c.kv_heads * kRows * 2 + part0 * dp + d;
-    const float ninf = -__builtin_inff();
-    // What a share's sum and outputs are multiplied by: one that saw nothing holds
-    // zeros (or NaN, which stays).
-    auto factor = [&](float m, float mm) { return m == ninf ? 1.0f : __builtin_amdgcn_exp2f(m - mm); };
-    if (used <= kJoinFew) {
-        for (uint32_t row = threadIdx.x / quads; row < count; row += kAttJoin / quads) {
-            if (threadIdx.x >= kAttJoin / quads * quads) break;  // lanes past the last whole row
-            float2 u[kJoinFew];
-            f32x4 w[kJoinFew];
+    j.used = (att_steps(att_limit(a, t, last_row)) + t.chunk - 1) / t.chunk;
+    j.dp = 32 * a.c.nb;
+    j.next = (uint64_t)a.c.kv_heads * kRows;
+    const uint64_t row0 = ((uint64_t)t.item * a.c.kv_heads + j.head) * kRows + j.from;
+    j.ml = reinterpret_cast<const float2*>(a.part) + row0;
+    j.out = a.part + (uint64_t)a.items * a.c.kv_heads * kRows * 2 + row0 * j.dp;
+    return j;
+}
+
+// Joins the shares of a tile: a thread has four dimensions of a row and goes over
+// the shares, kAhead of them in flight.
+template <uint32_t kRows>
+struct AttJoin {
+    static constexpr uint32_t kThreads = kRows <= 8 ? 128 : 256;
+    static constexpr uint32_t kParts = kRows <= 8 ? 1 : kRows / 16;  // workgroups of a tile
+    static constexpr int kAhead = 8;
+};
+
+template <uint32_t kRows>
+__global__ __launch_bounds__(AttJoin<kRows>::kThreads) void att_join_kernel(AttArgs a) {
+    constexpr int kAhead = AttJoin<kRows>::kAhead;
+    const JoinRows j = join_rows<kRows, AttJoin<kRows>::kParts>(a);
+    const uint32_t quads = j.dp / 4, at_once = AttJoin<kRows>::kThreads / quads;
+    if (j.count == 0 || threadIdx.x >= at_once * quads) return;
+    const uint32_t d = threadIdx.x % quads * 4;
+    for (uint32_t row = threadIdx.x / quads; row < j.count; row += at_once) {
+        const float ninf = -__builtin_inff();
+        float mm = ninf, ll = 0.0f;
+        f32x4 v = {0.f, 0.f, 0.f, 0.f};
+        for (uint32_t z0 = 0; z0 < j.used; z0 += kAhead) {
+            float2 u[kAhead];
+            f32x4 w[kAhead];
 #pragma unroll
-            for (uint32_t z = 0; z < kJoinFew; ++z) {
-                const uint32_t at = z < used ? z : 0;
-                u[z] = pm[at * next + row];
-                w[z] = *reinterpret_cast<const f32x4*>(po + (at * next + row) * dp);
+            for (int z = 0; z < kAhead; ++z) {
+                const uint64_t at = min(z0 + z, j.used - 1) * j.next + row;
+                u[z] = j.ml[at];
+                w[z] = *reinterpret_cast<const f32x4*>(j.out + at * j.dp + d);
             }
-            float mm = ninf, ll = 0.0f;
-            f32x4 v = {0.f, 0.f, 0.f, 0.f};
+            float top = mm;
 #pragma unroll
-            for (uint32_t z = 0; z < kJoinFew; ++z) mm = fmaxf(mm, u[z].x);
+            for (int z = 0; z < kAhead; ++z) top = fmaxf(top, u[z].x);
+            const float f0 = join_factor(mm, top);
+            mm = top;
+            ll *= f0;
+            v *= f0;
 #pragma unroll
-            for (uint32_t z = 0; z < kJoinFew; ++z)
-                if (z < used) {
-                    const float f = factor(u[z].x, mm);
+            for (int z = 0; z < kAhead; ++z)
+                if (z0 + z < j.used) {
+                    const float f = join_factor(u[z].x, mm);
                     ll += u[z].y * f;
                     v += w[z] * f;
                 }
-            join_store(a, t, head, t.first + from + row, d, ll, v);
         }
-        return;
+        join_store(a, j.t, j.head, j.t.first + j.from + row, d, ll, v);
     }
-    const uint32_t group = kJoinRows * quads, groups = kAttJoin / group;
-    const uint32_t gr = threadIdx.x / group, row = threadIdx.x % group / quads;
-    for (uint32_t row0 = 0; row0 < count; row0 += kJoinRows) {
-        __syncthreads();
-        // rows past the sequence's hold anything and are not stored
-        for (uint32_t i = threadIdx.x; i < used * kJoinRows; i += kAttJoin)
-            ml[i % kJoinRows][i / kJoinRows] = pm[i / kJoinRows * next + row0 + i % kJoinRows];
-        __syncthreads();
-        float mm = ninf, ll = 0.0f;
-        f32x4 v = {0.f, 0.f, 0.f, 0.f};
-        if (gr < groups) {
-            for (uint32_t z = 0; z < used; ++z) mm = fmaxf(mm, ml[row][z].x);
-            const float* p = po + (uint64_t)(row0 + row) * dp;
+}
+
+// The same for many shares of few tiles: a workgroup has one row, its threads the
+// shares' maxima and sums, then four dimensions and every kth share each.
+template <uint32_t kRows>
+__global__ __launch_bounds__(kAttBlock) void att_join_wide_kernel(AttArgs a) {
+    constexpr uint32_t kEach = kAttMaxSplits / kAttBlock;
+    __shared__ float factor[kAttMaxSplits], one[kAttWaves];
+    __shared__ f32x4 red[kAttBlock];
+    const JoinRows j = join_rows<kRows, kRows>(a);
+    if (j.count == 0) return;
+    const uint32_t wave = threadIdx.x / kWave;
+    const float ninf = -__builtin_inff();
+    float2 u[kEach];
+    float mm = ninf, ll = 0.0f;
+#pragma unroll
+    for (uint32_t k = 0; k < kEach; ++k) {
+        const uint32_t z = threadIdx.x + k * kAttBlock;
+        u[k] = z < j.used ? j.ml[z * j.next] : make_float2(ninf, 0.0f);
+        mm = fmaxf(mm, u[k].x);
+    }
+#pragma unroll
+    for (int x = 1; x < kWave; x *= 2) mm = fmaxf(mm, __shfl_xor(mm, x, kWave));
+    one[wave] = mm;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kAttWaves; ++w) mm = fmaxf(mm, one[w]);
+    __syncthreads();
+#pragma unroll
+    for (uint32_t k = 0; k < kEach; ++k) {
+        const float f = join_factor(u[k].x, mm);
+        factor[threadIdx.x + k * kAttBlock] = f;
+        ll += u[k].y * f;
+    }
+#pragma unroll
+    for (int x = 1; x < kWave; x *= 2) ll += __shfl_xor(ll, x, kWave);
+    one[wave] = ll;
+    __syncthreads();
+    ll = one[0];
+#pragma unroll
+    for (int w = 1; w < kAttWaves; ++w) ll += one[w];
+    const uint32_t quads = j.dp / 4, groups = kAttBlock / quads, gr = threadIdx.x / quads, d = threadIdx.x % quads * 4;
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+    if (gr < groups) {
 #pragma unroll 8
-            for (uint32_t z = gr; z < used; z += groups)
-                v += *reinterpret_cast<const f32x4*>(p + z * next * dp) * factor(ml[row][z].x, mm);
-        }
-        red[threadIdx.x] = v;
-        __syncthreads();
-        if (gr != 0 || row0 + row >= count) continue;
-        for (uint32_t k = 1; k < groups; ++k) v += red[threadIdx.x + k * group];
-        for (uint32_t z = 0; z < used; ++z) ll += ml[row][z].y * factor(ml[row][z].x, mm);
-        join_store(a, t, head, t.first + from + row0 + row, d, ll, v);
+        for (uint32_t z = gr; z < j.used; z += groups)
+            v += *reinterpret_cast<const f32x4*>(j.out + z * j.next * j.dp + d) * factor[z];
     }
+    red[threadIdx.x] = v;
+    __syncthreads();
+    if (gr != 0) return;
+    for (uint32_t k = 1; k < groups; ++k) v += red[threadIdx.x + k * quads];
+    join_store(a, j.t, j.head, j.t.first + j.from, d, ll, v);
 }
 
 // Rows of an item: a decode step's query heads in a few columns, or 32 for each of
@@ -869,6 +922,7 @@ __global__ __launch_bounds__(kAttJoin) void att_join_kernel(AttArgs a) {
 struct AttPlan {
     uint32_t rows;  // kRows: 4, 8 (kSlot), 64 or 128 (kSlot 16)
     uint32_t tiles, items, target;
+    bool wide;       // many shares of a tile
     uint64_t bytes;  // workspace
 };
 
@@ -884,6 +938,10 @@ struct AttPlan {
 // 96 of them: 108 us, cut 114; 4 x 256 tokens after 32768: 1031 -> 608 us.  Below
 // 2048 tokens the second kernel costs more than the shares save (1 x 1024: 10.4 us,
 // cut 12.1; 1 x 2048: 12.0 us, uncut 15.8).
+//
+// Join.  With more than 8 shares a tile a workgroup joins one row (1 x 131072, 8
+// query heads on 1: 145 -> 36 us); with fewer all rows of a tile do (45 x 8192: 48
+// us, 53 with a workgroup a row).
 static int att_plan(uint64_t num_seqs, uint64_t tokens, uint64_t q_heads, uint64_t kv_heads, uint64_t page_size,
                     uint64_t max_pages, uint32_t nb, AttPlan* p) {
     const uint64_t group = q_heads / kv_heads, rows = tokens * group;
@@ -901,6 +959,7 @@ static int att_plan(uint64_t num_seqs, uint64_t tokens, uint64_t q_heads, uint64
     p->target = cut ? (uint32_t)std::min<uint64_t>({std::max((want + kv_heads - 1) / kv_heads, 2 * busy),
                                                     tiles * shares, kAttMaxSplits})
                     : 0;
+    p->wide = p->target > 8 * tiles;
     p->tiles = (uint32_t)tiles;
     p->items = std::max((uint32_t)tiles, p->target);
     p->bytes = cut ? (uint64_t)p->items * kv_heads * p->rows * (2 + 32ull * nb) * 4 : 0;
@@ -920,26 +979,30 @@ static int att_check(uint64_t num_seqs, uint64_t tokens, uint64_t q_heads, uint6
     return att_plan(num_seqs, tokens, q_heads, kv_heads, page_size, max_pages, c->nb, p);
 }
 
-// join: the tiles whose shares are joined, or 0 for the items' kernel.
+enum class AttPass { kItems, kJoin, kJoinWide };
+
+// count: items or tiles.
 template <int NB, int R, int kSlot, int kPerSimd>
-static void att_launch_shape(const AttArgs& a, uint32_t join, dim3 grid, hipStream_t s) {
+static void att_launch_shape(const AttArgs& a, AttPass pass, uint32_t count, hipStream_t s) {
     constexpr uint32_t kRows = AttShape<NB, R, kSlot>::kRows;
-    if (join) {
-        grid = dim3(join * a.c.kv_heads * AttJoin<kRows>::kParts);
-        hipLaunchKernelGGL((att_join_kernel<kRows>), grid, dim3(kAttJoin), 0, s, a);
-    } else {
-        hipLaunchKernelGGL((att_kernel<NB, R, kSlot, kPerSimd>), grid, dim3(kAttBlock), 0, s, a);
-    }
+    const uint32_t x = count * a.c.kv_heads;
+    if (pass == AttPass::kItems)
+        hipLaunchKernelGGL((att_kernel<NB, R, kSlot, kPerSimd>), dim3(x), dim3(kAttBlock), 0, s, a);
+    else if (pass == AttPass::kJoin)
+        hipLaunchKernelGGL((att_join_kernel<kRows>), dim3(x * AttJoin<kRows>::kParts), dim3(AttJoin<kRows>::kThreads), 0,
+                           s, a);
+    else
+        hipLaunchKernelGGL((att_join_wide_kernel<kRows>), dim3(x * kRows), dim3(kAttBlock), 0, s, a);
 }
 
 // kPerSimd: the waves that a SIMD's registers hold.
-static void att_launch(const AttArgs& a, uint32_t rows, uint32_t join, dim3 grid, hipStream_t s) {
+static void att_launch(const AttArgs& a, uint32_t rows, AttPass pass, uint32_t count, hipStream_t s) {
     auto launch = [&](auto blocks) {
         constexpr int NB = decltype(blocks)::value;
-        if (rows == 4) att_launch_shape<NB, 1, 4, NB == 8 ? 2 : 3>(a, join, grid, s);
-        else if (rows == 8) att_launch_shape<NB, 1, 8, NB == 8 ? 1 : NB == 4 ? 3 : 4>(a, join, grid, s);
-        else if (rows == 64) att_launch_shape<NB, 1, 16, NB == 8 ? 1 : NB == 4 ? 2 : 3>(a, join, grid, s);
-        else if constexpr (NB < 8) att_launch_shape<NB, 2, 16, 2>(a, join, grid, s);
+        if (rows == 4) att_launch_shape<NB, 1, 4, NB == 8 ? 2 : 3>(a, pass, count, s);
+        else if (rows == 8) att_launch_shape<NB, 1, 8, NB == 8 ? 1 : NB == 4 ? 3 : 4>(a, pass, count, s);
+        else if (rows == 64) att_launch_shape<NB, 1, 16, NB == 8 ? 1 : NB == 4 ? 2 : 3>(a, pass, count, s);
+        else if constexpr (NB < 8) att_launch_shape<NB, 2, 16, 2>(a, pass, count, s);
     };
     if (a.c.nb <= 2) launch(std::integral_constant<int, 2>());
     else if (a.c.nb <= 4) launch(std::integral_constant<int, 4>());
@@ -1014,12 +1077,12 @@ extern "C" int kore_hip_attention_q4_f32(const float* q, const uint8_t* cache, c
     // A launch holds fewer than 2^32 threads: items in bands.
     const uint32_t band = (uint32_t)std::max<uint64_t>(1, 0x400000u / kv_heads);
     for (a.item0 = 0; a.item0 < p.items; a.item0 += band) {
-        att_launch(a, p.rows, 0, dim3(std::min(band, p.items - a.item0) * (uint32_t)kv_heads), (hipStream_t)stream);
+        att_launch(a, p.rows, AttPass::kItems, std::min(band, p.items - a.item0), (hipStream_t)stream);
         const int rc = launch_status();
         if (rc != KORE_HIP_OK) return rc;
     }
     if (p.target) {  // few tiles, or their keys would not be cut
-        att_launch(a, p.rows, p.tiles, dim3(), (hipStream_t)stream);
+        att_launch(a, p.rows, p.wide ? AttPass::kJoinWide : AttPass::kJoin, p.tiles, (hipStream_t)stream);
         return launch_status();
     }
     return KORE_HIP_OK;
