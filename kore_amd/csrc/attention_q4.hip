@@ -937,7 +937,10 @@ struct AttPlan {
 // holds at once.  45 decode steps over up to 8192 tokens, 8 key heads: 67 -> 53 us;
 // 96 of them: 108 us, cut 114; 4 x 256 tokens after 32768: 1031 -> 608 us.  Below
 // 2048 tokens the second kernel costs more than the shares save (1 x 1024: 10.4 us,
-// cut 12.1; 1 x 2048: 12.0 us, uncut 15.8).
+// cut 12.1; 1 x 2048: 12.0 us, uncut 15.8).  From 16384 tokens on up to twice as many
+// tiles are cut, finer, for sequences of very different lengths (3 x 1024 tokens
+// after 32768: 2211 -> 1487 us; 80 x 20000, 8 query heads a key head: 244 -> 206;
+// equal lengths lose 5 % at most: 190 x 17000 603 -> 631).
 //
 // Join.  With more than 8 shares a tile a workgroup joins one row (1 x 131072, 8
 // query heads on 1: 145 -> 36 us); with fewer all rows of a tile do (45 x 8192: 48
@@ -955,8 +958,9 @@ static int att_plan(uint64_t num_seqs, uint64_t tokens, uint64_t q_heads, uint64
     const uint64_t want = (p->rows == 4 && nb <= 4 ? 3 : 2) * kAttCus;  // workgroups that the chip holds at once
     const uint64_t busy = std::max(some, rows / p->rows);
     const uint64_t shares = max_pages * page_size / (kAttMinChunk * kAttStep);  // of the longest sequence
-    const bool cut = busy * kv_heads < want && shares >= 8;
-    p->target = cut ? (uint32_t)std::min<uint64_t>({std::max((want + kv_heads - 1) / kv_heads, 2 * busy),
+    const uint64_t more = shares >= 64 ? 2 : 1;
+    const bool cut = busy * kv_heads < more * want && shares >= 8;
+    p->target = cut ? (uint32_t)std::min<uint64_t>({std::max((want + kv_heads - 1) / kv_heads, 2 * more * busy),
                                                     tiles * shares, kAttMaxSplits})
                     : 0;
     p->wide = p->target > 8 * tiles;
