@@ -18,6 +18,7 @@
 // floats at 4l and the four at D/2 + 4l, so a half-split pair never leaves its
 // lane and the row's sums are all that crosses lanes.
 #include <algorithm>
+#include <initializer_list>
 
 #include "common.hpp"
 #include "kore_hip_internal.hpp"
@@ -443,6 +444,38 @@ static bool qk_outputs_alias(const QkArgs& a) {
                         (uint64_t)a.heads[1] * a.dim, a.tokens);
 }
 
+// Whether rows of a strided output meet `bytes` bytes at p.
+static bool qk_rows_meet(const float* y, uint64_t stride, uint64_t width, uint64_t n, const void* p, uint64_t bytes) {
+    if (!y || !p || !n || !width || !bytes) return false;
+    const uint64_t lo = (uint64_t)(uintptr_t)p, hi = lo + bytes, at = (uint64_t)(uintptr_t)y;
+    const uint64_t first = lo < at ? 0 : std::min((lo - at) / (stride * 4), n - 1);
+    for (uint64_t r = first; r < std::min(first + 2, n); ++r)
+        if (at + r * stride * 4 < hi && lo < at + (r * stride + width) * 4) return true;
+    return false;
+}
+
+struct QkFlat {
+    const void* p;
+    uint64_t bytes;
+};
+
+// Whether an output's rows meet what all rows read (weights, table, positions) or
+// one of `more`.
+static bool qk_meets(const QkArgs& a, std::initializer_list<QkFlat> more) {
+    const uint64_t row = (uint64_t)a.dim * 4;
+    for (int t = 0; t < 2; ++t) {
+        const uint64_t width = (uint64_t)a.heads[t] * a.dim;
+        auto meets = [&](const void* p, uint64_t bytes) {
+            return qk_rows_meet(a.y[t], a.ys[t], width, a.tokens, p, bytes);
+        };
+        if (meets(a.w[0], row) || meets(a.w[1], row) || meets(a.inv_freq, row / 2) || meets(a.positions, a.tokens * 4))
+            return true;
+        for (const QkFlat& f : more)
+            if (meets(f.p, f.bytes)) return true;
+    }
+    return false;
+}
+
 #define QK_LANES(L, CALL)                  \
     switch (L) {                           \
         case 1: { CALL(1); } break;        \
@@ -483,7 +516,7 @@ extern "C" int kore_hip_qk_norm_rope_f32(const float* q, const float* k, const f
     a.w[1] = k_weight;
     a.inv_freq = inv_freq;
     a.eps = eps;
-    if (qk_alias(a, a.x, a.xs, true) || qk_outputs_alias(a)) return KORE_HIP_ERR_ALIAS;
+    if (qk_alias(a, a.x, a.xs, true) || qk_outputs_alias(a) || qk_meets(a, {})) return KORE_HIP_ERR_ALIAS;
     hipStream_t s = (hipStream_t)stream;
     const bool vec = qk_vector(head_dim);
     const uint32_t lanes = qk_lanes(head_dim), rows = kQkBlock / std::min(lanes, 64u);
@@ -568,7 +601,19 @@ extern "C" int kore_hip_qk_norm_rope_backward_f32(
         a.eps = eps;
         a.part = workspace;
         for (int t = 0; t < 2; ++t) a.parts[t] = plan.parts[t];
-        if (qk_alias(a, a.x, a.xs, true) || qk_alias(a, a.dy, a.dys, true) || qk_outputs_alias(a))
+        const uint64_t dw = (uint64_t)head_dim * 4;
+        if (qk_alias(a, a.x, a.xs, true) || qk_alias(a, a.dy, a.dys, true) || qk_outputs_alias(a) ||
+            qk_meets(a, {{workspace, need}, {grad_q_weight, dw}, {grad_k_weight, dw}}))
+            return KORE_HIP_ERR_ALIAS;
+        const QkFlat flat[] = {{q_weight, dw}, {k_weight, dw}, {inv_freq, dw / 2}, {positions, a.tokens * 4},
+                               {grad_q_weight, dw}, {grad_k_weight, dw}};
+        for (const QkFlat& f : flat)
+            if (qk_rows_meet(workspace, need / 4, need / 4, 1, f.p, f.bytes)) return KORE_HIP_ERR_ALIAS;
+        for (int t = 0; t < 2; ++t)
+            if (a.heads[t] && (qk_rows_meet(a.x[t], a.xs[t], (uint64_t)a.heads[t] * head_dim, a.tokens, workspace, need) ||
+                               qk_rows_meet(a.dy[t], a.dys[t], (uint64_t)a.heads[t] * head_dim, a.tokens, workspace, need)))
+                return KORE_HIP_ERR_ALIAS;
+        if (q_heads && k_heads && qk_rows_meet(grad_q_weight, head_dim, head_dim, 1, grad_k_weight, dw))
             return KORE_HIP_ERR_ALIAS;
         const dim3 grid(plan.parts[0] + plan.parts[1]), block(kQkBwBlock);
         if (qk_vector(head_dim)) {
