@@ -442,8 +442,9 @@ int kore_hip_kv_cache_read_q4_f32(const uint8_t *cache, const uint32_t *slots,
  * 4-bit values are exact, scores, probabilities and sums f32.
  * The reference attends in f32 on the CPU (crates/kore-attention/src/flash.rs:28).
  * workspace (16-byte aligned): kore_hip_attention_q4_workspace_bytes bytes,
- * which may be 0; less is KORE_HIP_ERR_BAD_DIM.  Calls that may overlap in time
- * need workspaces of their own.  out overlaps no input (KORE_HIP_ERR_ALIAS). */
+ * which may be 0 and may be more for fewer tokens; less is KORE_HIP_ERR_BAD_DIM.
+ * Calls that may overlap in time need workspaces of their own.  Neither out nor
+ * the workspace overlaps an input or each other (KORE_HIP_ERR_ALIAS). */
 uint64_t kore_hip_attention_q4_workspace_bytes(uint64_t num_seqs,
                                                uint64_t tokens,
                                                uint64_t q_heads,

@@ -61,6 +61,7 @@ struct AttArgs {
     uint32_t num_seqs, q_heads, group, max_pages, dim;
     uint32_t items, item0;  // work items there can be (see att_item), first of this launch
     uint32_t target;        // items to cut the keys into, 0: one a tile
+    int search;             // many sequences: numbered with gaps, so that one can be found
     float scale_log2;
     int causal;
     Q4Cache c;
@@ -122,6 +123,30 @@ __device__ __forceinline__ AttItem att_item(const AttArgs& a, uint32_t number) {
         }
     };
     auto tiles = [&](int k) { return (len[k] * a.group + kRows - 1) / kRows; };
+    if (!kTiles && a.search) {
+        // Sequence s begins at number floor(starts[s] * group / kRows) + s, which leaves
+        // each as many numbers as it has tiles or more: found 64 sequences at a time.
+        auto begin = [&](uint32_t s) { return min(a.starts[s], lim) * a.group / kRows + s; };
+        uint32_t lo = 0;
+        for (uint32_t n = a.num_seqs; n;) {
+            const uint32_t each = (n + kWave - 1) / kWave, at = lane_id() * each;
+            const uint32_t below = (uint32_t)__popcll(__ballot(at < n && begin(lo + min(at, n - 1)) <= number));
+            if (below == 0) return t;  // before the first
+            lo += (below - 1) * each;
+            n = each == 1 ? 0 : min(each, n - (below - 1) * each);
+        }
+        t.q0 = min(a.starts[lo], lim);
+        t.q_len = max(min(a.starts[lo + 1], lim), t.q0) - t.q0;
+        t.kv_len = min(a.lens[lo], cap);
+        t.rows = t.q_len * a.group;
+        t.seq = lo;
+        t.splits = 1;
+        t.item = number;
+        const uint32_t tile = number - begin(lo), n = (t.rows + kRows - 1) / kRows;
+        t.ok = tile < n;
+        t.first = t.ok ? (n - 1 - tile) * kRows : 0;
+        return t;
+    }
     const bool one = a.num_seqs <= kHeld * kWave;
     if (one) read(0);
     t.chunk = kAttMaxSteps;  // a share a tile
@@ -923,6 +948,7 @@ struct AttPlan {
     uint32_t rows;  // kRows: 4, 8 (kSlot), 64 or 128 (kSlot 16)
     uint32_t tiles, items, target;
     bool wide;       // many shares of a tile
+    bool search;     // many sequences
     uint64_t bytes;  // workspace
 };
 
@@ -942,6 +968,10 @@ struct AttPlan {
 // after 32768: 2211 -> 1487 us; 80 x 20000, 8 query heads a key head: 244 -> 206;
 // equal lengths lose 5 % at most: 190 x 17000 603 -> 631).
 //
+// Search.  Every workgroup looks through the sequences up to its own, 256 at a time;
+// past 2048 it searches, in a numbering with gaps (4000 x 512: 1479 -> 711 us, 1000 x
+// 1024: 202 -> 233).
+//
 // Join.  With more than 8 shares a tile a workgroup joins one row (1 x 131072, 8
 // query heads on 1: 145 -> 36 us); with fewer all rows of a tile do (45 x 8192: 48
 // us, 53 with a workgroup a row).
@@ -953,13 +983,14 @@ static int att_plan(uint64_t num_seqs, uint64_t tokens, uint64_t q_heads, uint64
               : rows <= 16 * num_seqs || nb > 4 || rows / 128 * kv_heads <= 2 * kAttCus ? 64
                                                                                          : 128;
     const uint64_t some = std::min(num_seqs, tokens);  // sequences with new tokens, at most
-    const uint64_t tiles = rows / p->rows + some;
-    if (tiles > 0x3fffffull) return KORE_HIP_ERR_OVERFLOW;
     const uint64_t want = (p->rows == 4 && nb <= 4 ? 3 : 2) * kAttCus;  // workgroups that the chip holds at once
     const uint64_t busy = std::max(some, rows / p->rows);
     const uint64_t shares = max_pages * page_size / (kAttMinChunk * kAttStep);  // of the longest sequence
     const uint64_t more = shares >= 64 ? 2 : 1;
-    const bool cut = busy * kv_heads < more * want && shares >= 8;
+    const bool cut = busy * kv_heads < more * want && shares >= 8 && num_seqs <= 4096;
+    p->search = !cut && num_seqs > 2048;
+    const uint64_t tiles = rows / p->rows + (p->search ? num_seqs : some);
+    if (tiles > 0x3fffffull) return KORE_HIP_ERR_OVERFLOW;
     p->target = cut ? (uint32_t)std::min<uint64_t>({std::max((want + kv_heads - 1) / kv_heads, 2 * more * busy),
                                                     tiles * shares, kAttMaxSplits})
                     : 0;
@@ -1061,6 +1092,12 @@ extern "C" int kore_hip_attention_q4_f32(const float* q, const uint8_t* cache, c
         att_overlap(out, out_bytes, page_table, num_seqs * max_pages * 4) ||
         att_overlap(out, out_bytes, kv_lens, num_seqs * 4) || att_overlap(out, out_bytes, q_starts, num_seqs * 4 + 4))
         return KORE_HIP_ERR_ALIAS;
+    if (p.bytes && (att_overlap(workspace, p.bytes, q, ((tokens - 1) * a.q_stride + row) * 4) ||
+                    att_overlap(workspace, p.bytes, cache, bytes) ||
+                    att_overlap(workspace, p.bytes, page_table, num_seqs * max_pages * 4) ||
+                    att_overlap(workspace, p.bytes, kv_lens, num_seqs * 4) ||
+                    att_overlap(workspace, p.bytes, q_starts, num_seqs * 4 + 4)))
+        return KORE_HIP_ERR_ALIAS;
     a.q = q;
     a.cache = cache;
     a.table = page_table;
@@ -1076,6 +1113,7 @@ extern "C" int kore_hip_attention_q4_f32(const float* q, const uint8_t* cache, c
     a.dim = (uint32_t)head_dim;
     a.items = p.items;
     a.target = p.target;
+    a.search = p.search;
     a.scale_log2 = (float)((double)scale * 1.4426950408889634);
     a.causal = causal != 0;
     // A launch holds fewer than 2^32 threads: items in bands.

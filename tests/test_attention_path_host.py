@@ -98,6 +98,12 @@ def test_norm_rope_refusals():
     assert norm_rope(qo=P, qos=512) == ALIAS
     # rows of k inside the gaps of q's, but one float too far in
     assert norm_rope(q=P, qo=P, qs=512, qos=512, k=P + 4 * (4 * 64 - 1), ko=P + 4 * (4 * 64 - 1), ks=512, kos=512) == ALIAS
+    # outputs over what every row reads
+    row, end = 4 * 64 * 4, 6 * 4 * 64 * 4
+    for name, size in (("qw", 256), ("kw", 256), ("inv", 128), ("pos", 24)):
+        assert norm_rope(**{name: P + 2 * M}) == norm_rope(**{name: P + 2 * M + end - 4}) == ALIAS, name
+        assert norm_rope(**{name: P + 3 * M - 4}) == norm_rope(**{name: P + 3 * M + 64}) == ALIAS, name
+        assert norm_rope(**{name: P + 2 * M + 5 * 2 * row - 4}, qos=512) == ALIAS, name  # the last token's row
 
 
 def norm_rope_bwd(dq=P, dk=P + M, q=P + 2 * M, k=P + 3 * M, qw=P + 8 * M, kw=P + 8 * M, inv=P + 9 * M, gq=P + 4 * M,
@@ -124,6 +130,12 @@ def test_norm_rope_backward_refusals():
         assert norm_rope_bwd(strides=s) == DIM, i
     assert norm_rope_bwd(gq=P + 5 * M + 4) == ALIAS and norm_rope_bwd(gq=P + M) == ALIAS and norm_rope_bwd(gk=P + 2 * M) == ALIAS
     assert norm_rope_bwd(gq=P + 4) == ALIAS
+    for name in ("qw", "kw", "inv", "gqw", "gkw"):
+        assert norm_rope_bwd(**{name: P + 4 * M + 64}) == norm_rope_bwd(**{name: P + 5 * M}) == ALIAS, name
+        assert norm_rope_bwd(**{name: P + 10 * M + 4}) == ALIAS, name
+    for name in ("dq", "dk", "q", "k", "gq", "gk"):
+        assert norm_rope_bwd(**{name: P + 10 * M - 4}) == ALIAS, name
+    assert norm_rope_bwd(gkw=P + 6 * M + 252) == ALIAS
     assert norm_rope_bwd(batch=2 ** 30, seq=1, wsb=2 ** 40) == OVER  # more than 32 bits of rows
     ws = lib.kore_hip_qk_norm_rope_backward_workspace_bytes
     assert ws(0, 4, 2, 64) == 0 and ws(5, 0, 0, 64) == 0 and ws(1, 1, 1, 64) == 512 and ws(1, 3, 0, 64) == 256
@@ -180,5 +192,7 @@ def test_attention_refusals():
     assert need > 0
     assert attention(most=1024, wsb=need - 1) == DIM and attention(most=1024, ws=None) == NULL
     assert attention(most=1024, ws=P + 8 * M + 4) == DIM and attention(most=1024, out=P + 8 * M) == ALIAS
+    for name in ("q", "cache", "table", "lens", "starts"):
+        assert attention(most=1024, **{name: P + 8 * M}) == ALIAS, name
     assert lib.kore_hip_attention_q4_workspace_bytes(2, 5, 4, 3, 64, 16, 1024) == 0
     assert lib.kore_hip_attention_q4_workspace_bytes(2, 0, 4, 2, 64, 16, 1024) == 0

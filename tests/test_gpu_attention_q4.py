@@ -89,6 +89,23 @@ def test_split_contexts(hq, hk, d, page, lens, news):
     c.check(causal=False)
 
 
+@pytest.mark.parametrize("seqs,hq,hk,d,most,first,news", [(400, 8, 4, 32, 40, 3, [1]), (300, 18, 6, 64, 20, 0, [0, 1, 2, 40]), (5000, 3, 1, 16, 3, 0, [0, 0, 1]),
+                                                          (257, 24, 8, 16, 40, 1, [9, 0]), (2300, 4, 2, 16, 8, 7, [1]), (2100, 6, 3, 16, 4, 0, [0, 35, 2])])
+def test_many_sequences(seqs, hq, hk, d, most, first, news):
+    """More sequences than a wave looks at in one go, some of them empty, rows before the first and behind the last."""
+    r = np.random.default_rng(seqs)
+    c = Case(hq, hk, d, 16, [int(x) for x in r.integers(0, most, seqs)], (news * seqs)[:seqs], seed=seqs)
+    c.starts = c.starts + np.uint32(first)
+    c.tokens += first + 2
+    c.q = normal((c.tokens, hq, d), seqs)
+    for causal in (True, False):
+        out = HipBuffer.from_host(DEV, np.full(c.q.size * 4, 0xFF, np.uint8))
+        c.run(causal, out)
+        got = out.to_host(np.float32).reshape(c.q.shape)
+        want, tol = q4_ref.attention(c.q, c.cache, c.table, c.lens, c.starts, c.scale, causal, np.full(c.q.shape, np.nan))
+        q4_ref.assert_within(got, want, tol)
+
+
 def test_table_longer_than_the_sequences():
     """A table sized for long contexts in front of short ones: most splits have nothing to do."""
     c = Case(4, 2, 64, 16, [5, 40, 0], [1, 1, 1], seed=4, spare=2000)
