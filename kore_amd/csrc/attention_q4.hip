@@ -32,12 +32,13 @@
 // Bound and measured (MI355X; a copy of 2 GiB moves 4.5 TB/s, one that the last cache
 // holds 8.2; a bf16 matrix product reaches 1402 TFLOP/s):
 //   decode, HBM: 2 sequences of 131072 and 70320 tokens, 8 key heads of 128, 219 MB:
-//     45.5 us (4.8 TB/s) and 7.1 to join; 45 of 8192 .. 2049, 256 MB: 54 and 5.2.
-//     The conversion and softmax of a step, some 185 vector instructions, take two
-//     thirds of that time beside the loads.
+//     45.5 us (4.8 TB/s) and 7.0 to join; 45 of 8192 .. 2048, 256 MB: 60 and 5.4.
+//     The conversion and softmax of a step, some 185 vector instructions, are issued
+//     in 70 % of the cycles beside the loads.
 //   one sequence of 2048 tokens: 7.6 + 4.2 us, two launches and their chains of loads.
 //   prompt, matrix cores: 4096 tokens, 32 + 8 heads of 128, 137 GFLOP of which each is
-//     three in bf16: 305 us, 1350 TFLOP/s in bf16.
+//     three in bf16: 305 us, 1350 TFLOP/s in bf16 (matrix cores busy in 60 % of the
+//     cycles, vector issue in 65 %).
 //   chunks of 1023 and fewer after 2777 and fewer, 16 heads of 64: 104 us, a third of
 //     it matrix cores: at 64 dimensions a step of a wave has 180 vector instructions
 //     for 24 products, and their issue bounds it (68 % of all cycles).
