@@ -264,3 +264,73 @@ def test_small_buffers_are_refused():
     c.table = np.zeros((1, 400), np.uint32)
     with pytest.raises(RocmError, match="invalid dimension"):
         c.run(workspace=HipBuffer.empty(DEV, 64))
+
+
+@pytest.mark.parametrize("page,lens,news", [(65536, [70, 300], [1, 3]), (4096, [4100, 17], [1, 1]), (1024, [1025, 2049, 5], [60, 1, 5])])
+def test_large_pages(page, lens, news):
+    Case(4, 2, 32, page, lens, news, seed=16).check()
+
+
+def test_sequences_that_share_pages():
+    """A common beginning cached once: the same pages in several rows of the table, and the whole table of one row twice."""
+    c = Case(6, 2, 64, 16, [64, 75, 90], [1, 2, 1], seed=17)
+    c.table[0, :4] = c.table[2, :4]
+    c.table[1, :3] = c.table[2, :3]
+    c.check()
+    c.table[1], c.lens[1] = c.table[2], c.lens[2]
+    c.check()
+    c.table[2, 1] = c.table[2, 0]  # one page at two places
+    c.check()
+
+
+def test_nothing_cached_and_nothing_new():
+    c = Case(4, 2, 64, 16, [20, 30], [2, 1], seed=18)
+    for pages, most in ((0, c.most), (c.cache.bytes.shape[0], 0), (0, 0)):
+        out = HipBuffer.from_host(DEV, np.full(c.q.size * 4, 0xFF, np.uint8))
+        rocm.rocm_attention_q4_f32(DEV, up(c.q), up(c.cache.bytes), up(c.table), up(c.lens), up(c.starts), 2, c.tokens, 4, 2, 64, pages, 16,
+                                   most, c.scale, True, 0, None, out)
+        assert (out.to_host(np.float32) == 0).all(), (pages, most)
+    for starts in ([0, 0, 0], [3, 3, 3], [99, 99, 99]):
+        out = HipBuffer.from_host(DEV, np.full(c.q.size * 4, 0xFF, np.uint8))
+        rocm.rocm_attention_q4_f32(DEV, up(c.q), up(c.cache.bytes), up(c.table), up(c.lens), up(np.array(starts, np.uint32)), 2, c.tokens, 4, 2,
+                                   64, c.cache.bytes.shape[0], 16, c.most, c.scale, True, 0, None, out)
+        assert (out.to_host(np.uint8) == 0xFF).all(), starts
+
+
+def test_two_calls_at_once():
+    """Two calls on two streams, over one cache and with workspaces of their own, many times over."""
+    c = Case(8, 2, 64, 16, [2600, 900], [1, 1], seed=19)
+    n = rocm.rocm_attention_q4_workspace_bytes(2, 2, 8, 2, 64, 16, c.most)
+    assert n > 0
+    b = [up(c.cache.bytes), up(c.table), up(c.lens), up(c.starts)]
+    qs = [normal(c.q.shape, 20 + i) for i in range(2)]
+    each = [(up(q), HipBuffer.empty(DEV, n), HipBuffer.empty(DEV, q.nbytes), torch.cuda.Stream()) for q in qs]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for q, ws, out, stream in each:
+            with torch.cuda.stream(stream):
+                rocm.rocm_attention_q4_f32(DEV, q, *b, 2, 2, 8, 2, 64, c.cache.bytes.shape[0], 16, c.most, c.scale, True, 0, ws, out)
+    torch.cuda.synchronize()
+    for q, (_, _, out, _) in zip(qs, each):
+        want, tol = q4_ref.attention(q, c.cache, c.table, c.lens, c.starts, c.scale, True, np.zeros(q.shape))
+        q4_ref.assert_within(out.to_host(np.float32).reshape(q.shape), want, tol)
+
+
+def test_offsets_past_32_bits():
+    """Pages past 4 GiB of the cache, and query rows 4 GiB apart: the same bits as from a small cache and dense rows."""
+    hq, hk, d, page, lens = 4, 2, 256, 64, [70, 150]
+    c = Case(hq, hk, d, page, lens, [1, 2], seed=21)
+    small = c.run(out=None).to_host(np.float32)[:c.q.size]
+    each = c.cache.bytes[0].nbytes
+    far = (1 << 32) // each + 1
+    cache = torch.empty(((far + c.cache.bytes.shape[0]) * each,), dtype=torch.uint8, device="cuda")
+    cache[far * each:].copy_(torch.from_numpy(c.cache.bytes.reshape(-1)))
+    cache[:c.cache.bytes.nbytes].fill_(0xFF)  # what a wrapped offset would meet
+    stride = 1 << 30
+    q = torch.empty(((c.tokens - 1) * stride + hq * d,), device="cuda")
+    for t in range(c.tokens):
+        q[t * stride:t * stride + hq * d].copy_(torch.from_numpy(c.q[t].reshape(-1)))
+    got = rocm.rocm_attention_q4_f32(DEV, HipBuffer.from_tensor(q), HipBuffer.from_tensor(cache), up(c.table + np.uint32(far)), up(c.lens), up(c.starts),
+                                     2, c.tokens, hq, hk, d, far + c.cache.bytes.shape[0], page, c.most, c.scale, True, stride)
+    torch.cuda.synchronize()
+    assert got.to_host(np.float32)[:c.q.size].tobytes() == small.tobytes()

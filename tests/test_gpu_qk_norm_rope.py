@@ -182,3 +182,45 @@ def test_capture_of_forward_and_backward():
         step()
         torch.cuda.synchronize()
         assert [o.to_host().tobytes() for o in outs] == want
+
+
+@pytest.mark.parametrize("start", [2 ** 20, 2 ** 32 + 5])
+def test_far_positions_without_a_table(start):
+    """Positions past 32 bits and far past an f32's exact integers."""
+    t, hq, hk, d = 5, 2, 1, 64
+    q, k = normal((t, hq, d), 30), normal((t, hk, d), 31)
+    w, inv = normal((d,), 32, 1.0, 0.1), rocm.rope_inv_freq_host(d, 10000.0)
+    pos = start + np.arange(t)
+    qo, ko = rocm.rocm_qk_norm_rope_f32(DEV, up(q), up(k), up(w), up(w), up(inv), 1, t, hq, hk, d, EPS, start)
+    for got, x in ((qo, q), (ko, k)):
+        want, tol = q4_ref.qk_norm_rope(x, w, pos, inv, EPS, False)
+        q4_ref.assert_within(got.to_host(np.float32).reshape(x.shape), want, tol)
+
+
+def test_two_backward_calls_at_once():
+    """On two streams with workspaces of their own: each the same bits as alone."""
+    t, hq, hk, d = 700, 4, 2, 64
+    n = rocm.rocm_qk_norm_rope_backward_workspace_bytes(t, hq, hk, d)
+    w, inv = up(normal((d,), 40, 1.0, 0.1)), up(rocm.rope_inv_freq_host(d, 10000.0))
+    calls = []
+    for i in range(2):
+        a = [up(normal((t, h, d), 41 + 10 * i + j)) for j, h in enumerate((hq, hk, hq, hk))]
+        out = dict(grad_q=HipBuffer.empty(DEV, t * hq * d * 4), grad_k=HipBuffer.empty(DEV, t * hk * d * 4), workspace=HipBuffer.empty(DEV, n))
+        calls.append((a, out, torch.cuda.Stream()))
+
+    def run(a, out):
+        return rocm.rocm_qk_norm_rope_backward_f32(DEV, *a, w, w, inv, 1, t, hq, hk, d, EPS, **out)
+
+    want = []
+    for a, out, _ in calls:
+        r = run(a, out)
+        torch.cuda.synchronize()
+        want.append([b.tensor().clone() for b in r])
+    for _ in range(10):
+        got = []
+        for a, out, stream in calls:
+            with torch.cuda.stream(stream):
+                got.append(run(a, out))
+        torch.cuda.synchronize()
+        for g, x in zip(got, want):
+            assert all(torch.equal(b.tensor()[:y.numel()], y) for b, y in zip(g, x))
