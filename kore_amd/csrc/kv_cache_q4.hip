@@ -15,11 +15,13 @@
 // a group side by side, so a workgroup takes neighbouring tokens and the L2
 // merges their stores.
 //
-// 8192 tokens of 8 heads of 128, K and V, 76 MB: written in 15.5 us (4.9 TB/s),
-// read back in 17.8 (a copy of as many bytes, held by the last cache, takes 10.5).
-// Four tokens a lane with one 16-byte store of V's codes: both together 39.7 us
-// where this takes 34.3 (four times fewer waves in flight); workgroups of 512 or
-// 1024 and loads past the caches made no difference.
+// 8192 tokens of 8 heads of 128, K and V, 76 MB: written in 15.4 .. 17.9 us (4.9 ..
+// 4.3 TB/s, by what the caches hold), read back in 15.2 (5.0; with a lane's eight
+// values on end and stores past the caches 17.9); a copy of as many bytes that the
+// last cache holds takes 10.5.  Four tokens a lane with one 16-byte store of V's
+// codes: both together 39.7 us where this takes 33.2 (four times fewer waves in
+// flight); workgroups of 512 or 1024, loads past the caches and the reading's lanes
+// for the writing made no difference.
 #include <algorithm>
 
 #include "q4.hpp"
@@ -114,45 +116,44 @@ __global__ __launch_bounds__(kQ4Block) void q4_write_kernel(Q4Args a) {
             (uint8_t)(finite ? (uint32_t)(e + 127) : kQ4NanScale);
 }
 
+// A lane has dimensions 4q .. 4q + 3 and 16 + 4q .. of its block, q its place among the
+// block's four lanes: each of its two stores and its neighbours' are 64 bytes on end.
 __global__ __launch_bounds__(kQ4Block) void q4_read_kernel(Q4Args a) {
     const uint32_t i = blockIdx.x * kQ4Block + threadIdx.x;
     const int which = blockIdx.y;
     if (i >= a.items) return;
     uint64_t token;
-    uint32_t head, chunk;
-    q4_item(a, i, &token, &head, &chunk);
+    uint32_t head, at;
+    q4_item(a, i, &token, &head, &at);
+    const uint32_t block = at >> 2, q = at & 3u;
     const uint32_t slot = a.slots[token];
     const uint32_t page = slot >> a.c.shift, t = slot & (a.c.page - 1u);
-    const uint32_t d0 = chunk * 8u;
-    if (d0 >= a.head_dim) return;
-    uint32_t code = 0, b = 127;
+    uint32_t code[2] = {0, 0}, b = 127;
     if (page < a.c.num_pages) {
         const uint8_t* base = a.cache + (uint64_t)page * a.c.page_bytes + (uint64_t)head * a.c.head_bytes;
-        code = *reinterpret_cast<const uint32_t*>(base + (which ? q4_v_code(a.c, t, chunk) : q4_k_code(a.c, t, chunk)));
-        b = base[which ? q4_v_scale(a.c, t, chunk >> 2) : q4_k_scale(a.c, t, chunk >> 2)];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const uint32_t chunk = 4 * block + 2 * h + (q >> 1);
+            code[h] = *reinterpret_cast<const uint16_t*>(
+                base + (which ? q4_v_code(a.c, t, chunk) : q4_k_code(a.c, t, chunk)) + 2 * (q & 1u));
+        }
+        b = base[which ? q4_v_scale(a.c, t, block) : q4_k_scale(a.c, t, block)];
     }
     const float s = b == kQ4NanScale ? __uint_as_float(0x7fc00000u) : q4_scale(b);
-    f32x4 v[2];
-    auto p = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(code, 1.0f, 0);
-    v[0].x = p[0] * s;
-    v[0].y = p[1] * s;
-    p = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(code, 1.0f, 1);
-    v[0].z = p[0] * s;
-    v[0].w = p[1] * s;
-    p = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(code, 1.0f, 2);
-    v[1].x = p[0] * s;
-    v[1].y = p[1] * s;
-    p = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(code, 1.0f, 3);
-    v[1].z = p[0] * s;
-    v[1].w = p[1] * s;
     float* row = a.out[which] + (token * a.c.kv_heads + head) * a.head_dim;
-    if (d0 + 8u <= a.head_dim) {
-        __builtin_nontemporal_store((f32x4_a4)v[0], reinterpret_cast<f32x4_a4*>(row + d0));
-        __builtin_nontemporal_store((f32x4_a4)v[1], reinterpret_cast<f32x4_a4*>(row + d0 + 4));
-    } else {
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-            if (d0 + j < a.head_dim) row[d0 + j] = v[j >> 2][j & 3];
+    for (int h = 0; h < 2; ++h) {
+        const uint32_t d = 32 * block + 16 * h + 4 * q;
+        const auto lo = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(code[h], 1.0f, 0);
+        const auto hi = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(code[h], 1.0f, 1);
+        const f32x4 v = {lo[0] * s, lo[1] * s, hi[0] * s, hi[1] * s};
+        if (d + 4u <= a.head_dim) {
+            *reinterpret_cast<f32x4_a4*>(row + d) = (f32x4_a4)v;
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (d + j < a.head_dim) row[d + j] = v[j];
+        }
     }
 }
 
