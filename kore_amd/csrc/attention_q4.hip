@@ -467,7 +467,13 @@ struct AttShape {
 // group g (K's codes as they lie, 16 bytes at head_dim 128; which eight of them
 // meet in one product is free, q's operand is taken alike) and gets tokens 4g ..
 // 4g + 3 of row n, for two tiles; for O^T those are its eight tokens.
-template <int NB, int R, int kSlot, int kPerSimd>
+//
+// kRaise: a wave's products go before other waves' softmax (s_setprio).  45 x 8192, 4
+// query heads on each of 8 key heads: 52.3 -> 50.9 us, 8 on each of 64 sequences 78 ->
+// 73; 64-row items after long contexts 5 .. 8 % (512 after 4096: 157 -> 148), but not 16
+// rows a sequence (65 -> 71) nor prompts of their own keys (1024: 37 -> 40), nor 256
+// dimensions (152 -> 171).  A branch on it would cost as much as it gives.
+template <int NB, int R, int kSlot, int kPerSimd, bool kRaise>
 __global__ __launch_bounds__(kAttBlock) __attribute__((amdgpu_waves_per_eu(kPerSimd, kPerSimd)))
 void att_kernel(AttArgs a) {
     using Shape = AttShape<NB, R, kSlot>;
@@ -496,10 +502,6 @@ void att_kernel(AttArgs a) {
     const uint32_t min_limit = att_limit(a, t, min(r0, t.rows - 1));
     const uint32_t end = r0 < r1 ? min(hi, att_steps(att_limit(a, t, r1 - 1))) : 0;
 
-    // Products before other waves' softmax: 8192 x 45, 8 key heads of 128, 4 query
-    // heads each 52.3 -> 50.9 us, 8 each (64 sequences) 78 -> 73; with 16-row columns
-    // 16 rows a sequence lost (65 -> 71 us) what long chunks gained (106 -> 99).
-    constexpr bool kRaise = kSlot < 16 && NB < 8;
     // q's third term lies in LDS where the registers would not hold it (4 x 4096
     // tokens, 32 + 8 heads of 128: 1295 -> 1193 us, the spills gone).
     constexpr bool kPark = kSlot == 16 && R == 2 && NB == 4;
@@ -965,6 +967,7 @@ struct AttPlan {
     uint32_t tiles, items, target;
     bool wide;       // many shares of a tile
     bool search;     // many sequences
+    bool raise;      // 64-row items: most keys are older than the new tokens
     uint64_t bytes;  // workspace
 };
 
@@ -1011,6 +1014,7 @@ static int att_plan(uint64_t num_seqs, uint64_t tokens, uint64_t q_heads, uint64
                                                     tiles * shares, kAttMaxSplits})
                     : 0;
     p->wide = p->target > 8 * tiles;
+    p->raise = rows > 16 * num_seqs && nb <= 4 && 2 * tokens < num_seqs * max_pages * page_size;
     p->tiles = (uint32_t)tiles;
     p->items = std::max((uint32_t)tiles, p->target);
     p->bytes = cut ? (uint64_t)p->items * kv_heads * p->rows * (2 + 32ull * nb) * 4 : 0;
@@ -1033,12 +1037,12 @@ static int att_check(uint64_t num_seqs, uint64_t tokens, uint64_t q_heads, uint6
 enum class AttPass { kItems, kJoin, kJoinWide };
 
 // count: items or tiles.
-template <int NB, int R, int kSlot, int kPerSimd>
+template <int NB, int R, int kSlot, int kPerSimd, bool kRaise = kSlot < 16 && NB < 8>
 static void att_launch_shape(const AttArgs& a, AttPass pass, uint32_t count, hipStream_t s) {
     constexpr uint32_t kRows = AttShape<NB, R, kSlot>::kRows;
     const uint32_t x = count * a.c.kv_heads;
     if (pass == AttPass::kItems)
-        hipLaunchKernelGGL((att_kernel<NB, R, kSlot, kPerSimd>), dim3(x), dim3(kAttBlock), 0, s, a);
+        hipLaunchKernelGGL((att_kernel<NB, R, kSlot, kPerSimd, kRaise>), dim3(x), dim3(kAttBlock), 0, s, a);
     else if (pass == AttPass::kJoin)
         hipLaunchKernelGGL((att_join_kernel<kRows>), dim3(x * AttJoin<kRows>::kParts), dim3(AttJoin<kRows>::kThreads), 0,
                            s, a);
@@ -1049,12 +1053,15 @@ static void att_launch_shape(const AttArgs& a, AttPass pass, uint32_t count, hip
 // kPerSimd: the waves that a SIMD's registers hold.  With one fewer 64-row items of 64
 // dimensions took 107 us where they take 96, 8-row ones 62 where 57 (45 x 8192, 40 + 8
 // heads of 96); one more spills.
-static void att_launch(const AttArgs& a, uint32_t rows, AttPass pass, uint32_t count, hipStream_t s) {
+static void att_launch(const AttArgs& a, const AttPlan& p, AttPass pass, uint32_t count, hipStream_t s) {
     auto launch = [&](auto blocks) {
         constexpr int NB = decltype(blocks)::value;
-        if (rows == 4) att_launch_shape<NB, 1, 4, NB == 8 ? 2 : 3>(a, pass, count, s);
-        else if (rows == 8) att_launch_shape<NB, 1, 8, NB == 8 ? 1 : NB == 4 ? 3 : 4>(a, pass, count, s);
-        else if (rows == 64) att_launch_shape<NB, 1, 16, NB == 8 ? 1 : NB == 4 ? 2 : 3>(a, pass, count, s);
+        constexpr int kMid = NB == 8 ? 1 : NB == 4 ? 2 : 3;
+        if (p.rows == 4) att_launch_shape<NB, 1, 4, NB == 8 ? 2 : 3>(a, pass, count, s);
+        else if (p.rows == 8) att_launch_shape<NB, 1, 8, NB == 8 ? 1 : NB == 4 ? 3 : 4>(a, pass, count, s);
+        else if (p.rows == 64 && p.raise && pass == AttPass::kItems)
+            att_launch_shape<NB, 1, 16, kMid, (NB < 8)>(a, pass, count, s);
+        else if (p.rows == 64) att_launch_shape<NB, 1, 16, kMid>(a, pass, count, s);
         else if constexpr (NB < 8) att_launch_shape<NB, 2, 16, 2>(a, pass, count, s);
     };
     if (a.c.nb <= 2) launch(std::integral_constant<int, 2>());
@@ -1137,12 +1144,12 @@ extern "C" int kore_hip_attention_q4_f32(const float* q, const uint8_t* cache, c
     // A launch holds fewer than 2^32 threads: items in bands.
     const uint32_t band = (uint32_t)std::max<uint64_t>(1, 0x400000u / kv_heads);
     for (a.item0 = 0; a.item0 < p.items; a.item0 += band) {
-        att_launch(a, p.rows, AttPass::kItems, std::min(band, p.items - a.item0), (hipStream_t)stream);
+        att_launch(a, p, AttPass::kItems, std::min(band, p.items - a.item0), (hipStream_t)stream);
         const int rc = launch_status();
         if (rc != KORE_HIP_OK) return rc;
     }
     if (p.target) {  // few tiles, or their keys would not be cut
-        att_launch(a, p.rows, p.wide ? AttPass::kJoinWide : AttPass::kJoin, p.tiles, (hipStream_t)stream);
+        att_launch(a, p, p.wide ? AttPass::kJoinWide : AttPass::kJoin, p.tiles, (hipStream_t)stream);
         return launch_status();
     }
     return KORE_HIP_OK;
