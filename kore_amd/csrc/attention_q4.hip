@@ -37,9 +37,9 @@
 //     in 70 % of the cycles beside the loads.
 //   one sequence of 2048 tokens: 7.6 + 4.2 us, two launches and their chains of loads.
 //   prompt, matrix cores: 4096 tokens, 32 + 8 heads of 128, 137 GFLOP of which each is
-//     three in bf16: 305 us, 1350 TFLOP/s in bf16 (matrix cores busy in 60 % of the
-//     cycles, vector issue in 65 %).
-//   chunks of 1023 and fewer after 2777 and fewer, 16 heads of 64: 104 us, a third of
+//     three in bf16: 306 .. 327 us by the card, 1350 .. 1260 TFLOP/s in bf16 (matrix
+//     cores busy in 60 % of the cycles, vector issue in 65 %).
+//   chunks of 1023 and fewer after 2777 and fewer, 16 heads of 64: 98 us, a third of
 //     it matrix cores: at 64 dimensions a step of a wave has 180 vector instructions
 //     for 24 products, and their issue bounds it (68 % of all cycles).
 #include <algorithm>
