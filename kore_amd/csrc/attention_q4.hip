@@ -183,7 +183,9 @@ __device__ __forceinline__ AttItem att_item(const AttArgs& a, uint32_t number) {
         // between all / target and all / (target - n).
         if (count < a.target) {
             const uint64_t most = (all + a.target - count - 1) / (a.target - count);
-            uint64_t chunk = max(one ? (all + a.target - 1) / a.target : most, (uint64_t)kAttMinChunk);
+            // at least: a 32nd of the average keys, from 8 steps to 32
+            const uint64_t least = kAttMinChunk * (all >= 1024ull * count ? 4 : all >= 512ull * count ? 2 : 1);
+            uint64_t chunk = max(one ? (all + a.target - 1) / a.target : most, least);
             while (chunk < most) {  // the sequences are in registers
                 uint64_t n = 0;     // shares
 #pragma unroll
@@ -765,8 +767,8 @@ void att_kernel(AttArgs a) {
         }
         return;
     }
-    // Join the waves of a group: to the common maximum, then add (and the second
-    // term's column to the first's).
+    // Join the waves of a group: to the common maximum, then add (and the terms'
+    // columns to the first's).
     __shared__ float sm[kAttWaves][16], sl[kAttWaves][16];
     auto& so = shared.so;
 #pragma unroll
@@ -986,6 +988,10 @@ struct AttPlan {
 // tiles are cut, finer, for sequences of very different lengths (3 x 1024 tokens
 // after 32768: 2211 -> 1487 us; 80 x 20000, 8 query heads a key head: 244 -> 206;
 // equal lengths lose 5 % at most: 190 x 17000 603 -> 631).
+//
+// Share.  At least 8 steps, two for each wave, and 16 or 32 of long sequences (worked
+// out from the lengths, att_item): 1 x 2048 11.3 us (16: 12.5), 1 x 16384 17.0 (16:
+// 14.9), 1 x 65536 26.7 (32: 24.4; 48: 24.8).
 //
 // Search.  Every workgroup looks through the sequences up to its own, 256 at a time;
 // past 2048 it searches, in a numbering with gaps (4000 x 512: 1479 -> 711 us, 1000 x
