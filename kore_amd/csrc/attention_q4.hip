@@ -113,10 +113,9 @@ __device__ __forceinline__ uint32_t att_steps(uint32_t keys) { return (keys + kA
 // kRows) tiles of ceil(steps / chunk) shares each.  The chunk is the same for all
 // sequences, so that items take equally long however ragged the lengths are: the
 // least (to an eighth; for more sequences than a wave's lanes hold, to a half) with
-// which there are no more than `target`.  The host
-// knows no lengths; the grid has as many items as there can be, and those past
-// the last are empty.  kTiles: `number` is that of a tile, and its first item is
-// meant.
+// which there are no more than `target`.  The host knows no lengths; the grid has as
+// many items as there can be, and those past the last are empty.  kTiles: `number` is
+// that of a tile, and its first item is meant.
 template <uint32_t kRows, bool kTiles>
 __device__ __forceinline__ AttItem att_item(const AttArgs& a, uint32_t number) {
     constexpr int kHeld = 4;  // sequences that a lane holds
@@ -962,8 +961,6 @@ __global__ __launch_bounds__(kAttBlock) void att_join_wide_kernel(AttArgs a) {
     join_store(a, j.t, j.head, j.t.first + j.from, d, ll, v);
 }
 
-// Rows of an item: a decode step's query heads in a few columns, or 32 for each of
-// four waves.
 struct AttPlan {
     uint32_t rows;  // kRows: 4, 8 (kSlot), 64 or 128 (kSlot 16)
     uint32_t tiles, items, target;
