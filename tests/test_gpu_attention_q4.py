@@ -106,6 +106,15 @@ def test_many_sequences(seqs, hq, hk, d, most, first, news):
         q4_ref.assert_within(got, want, tol)
 
 
+@pytest.mark.parametrize("hq,hk,d,lens,news", [(4, 2, 64, [30, 300, 5, 200, 17], [1, 150, 1, 90, 1]), (8, 2, 128, [2500, 40, 2100], [1, 40, 100]),
+                                               (6, 3, 32, [3000] + [20] * 90 + [260], [1] * 91 + [200])])
+def test_decode_steps_beside_chunks(hq, hk, d, lens, news):
+    """Sequences of one tile among those of several, uncut and cut."""
+    c = Case(hq, hk, d, 16, lens, news, seed=22)
+    c.check()
+    c.check(causal=False)
+
+
 def test_table_longer_than_the_sequences():
     """A table sized for long contexts in front of short ones: most splits have nothing to do."""
     c = Case(4, 2, 64, 16, [5, 40, 0], [1, 1, 1], seed=4, spare=2000)
