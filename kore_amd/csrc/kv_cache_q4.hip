@@ -9,19 +9,19 @@
 // nearest magnitude, ties to the even code.
 //
 // Bound: HBM.  A value costs 4 bytes of f32 and 17/32 of a byte in the cache.
-// One lane takes eight values (32 bytes in, one dword of codes out), so a
-// block's largest magnitude is a maximum over four lanes (two DPP moves).  K's
-// dwords are contiguous over a wave; V's lie 16 bytes apart, the four tokens of
-// a group side by side, so a workgroup takes neighbouring tokens and the L2
+// One lane takes eight values of a block, 4q .. 4q + 3 and 16 + 4q .. for its place q
+// among the block's four lanes: each of its two loads or stores of f32 is part of 64
+// bytes on end, and a block's largest magnitude is a maximum over four lanes (two DPP
+// moves).  K's codes are contiguous over a wave; V's lie 16 bytes apart, the four
+// tokens of a group side by side, so a workgroup takes neighbouring tokens and the L2
 // merges their stores.
 //
-// 8192 tokens of 8 heads of 128, K and V, 76 MB: written in 15.4 .. 17.9 us (4.9 ..
-// 4.3 TB/s, by what the caches hold), read back in 15.2 (5.0; with a lane's eight
-// values on end and stores past the caches 17.9); a copy of as many bytes that the
-// last cache holds takes 10.5.  Four tokens a lane with one 16-byte store of V's
-// codes: both together 39.7 us where this takes 33.2 (four times fewer waves in
-// flight); workgroups of 512 or 1024, loads past the caches and the reading's lanes
-// for the writing made no difference.
+// 8192 tokens of 8 heads of 128, K and V, 76 MB each way, among other work: written and
+// read back in 33.5 us; with a lane's eight values on end 35.0.  What is read back goes
+// past the caches (else 36.6; alone in a loop 33.2, where this takes 34.3), what is
+// written is not read past them (38.9).  Four tokens a lane with one 16-byte store of
+// V's codes 39.7 (four times fewer waves in flight); workgroups of 512 or 1024 made no
+// difference.  A copy of as many bytes that the last cache holds takes 10.5 each way.
 #include <algorithm>
 
 #include "q4.hpp"
@@ -55,12 +55,12 @@ __device__ __forceinline__ uint32_t divide(uint32_t i, uint32_t d, uint32_t inv,
     return q + (r >= d ? 1u : 0u);
 }
 
-// Item i -> token, key head, chunk of eight dimensions.
-__device__ __forceinline__ void q4_item(const Q4Args& a, uint32_t i, uint64_t* token, uint32_t* head, uint32_t* chunk) {
+// Item i -> token, key head, lane of the head (four a block).
+__device__ __forceinline__ void q4_item(const Q4Args& a, uint32_t i, uint64_t* token, uint32_t* head, uint32_t* lane) {
     const uint32_t chunks = 4u * a.c.nb;
     uint32_t in_row;
     *token = divide(i, chunks * a.c.kv_heads, a.per_row, &in_row);
-    *head = divide(in_row, chunks, a.per_chunks, chunk);
+    *head = divide(in_row, chunks, a.per_chunks, lane);
 }
 
 __global__ __launch_bounds__(kQ4Block) void q4_write_kernel(Q4Args a) {
@@ -68,22 +68,23 @@ __global__ __launch_bounds__(kQ4Block) void q4_write_kernel(Q4Args a) {
     const int which = blockIdx.y;  // 0: K, 1: V
     if (i >= a.items) return;      // whole blocks of four lanes leave
     uint64_t token;
-    uint32_t head, chunk;
-    q4_item(a, i, &token, &head, &chunk);
+    uint32_t head, lane;
+    q4_item(a, i, &token, &head, &lane);
+    const uint32_t block = lane >> 2, q = lane & 3u;
     const float* row = a.in[which] + token * a.stride[which] + (uint64_t)head * a.head_dim;
-    const uint32_t d0 = chunk * 8u;
+    const uint32_t slot = a.slots[token];
     float x[8];
-    if (d0 + 8u <= a.head_dim) {
-        const f32x4 lo = *reinterpret_cast<const f32x4_a4*>(row + d0);
-        const f32x4 hi = *reinterpret_cast<const f32x4_a4*>(row + d0 + 4);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            x[j] = lo[j];
-            x[4 + j] = hi[j];
+    for (int h = 0; h < 2; ++h) {
+        const uint32_t d = 32 * block + 16 * h + 4 * q;
+        if (d + 4u <= a.head_dim) {
+            const f32x4 v = *reinterpret_cast<const f32x4_a4*>(row + d);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[4 * h + j] = v[j];
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[4 * h + j] = d + j < a.head_dim ? row[d + j] : 0.0f;
         }
-    } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = d0 + j < a.head_dim ? row[d0 + j] : 0.0f;
     }
     // The bits of |x| are ordered as their values, infinities and NaN last.
     uint32_t amax = 0;
@@ -97,35 +98,35 @@ __global__ __launch_bounds__(kQ4Block) void q4_write_kernel(Q4Args a) {
     // 6 is the largest code; 3 * 2^126 the largest magnitude that the top scale holds
     // without overflow.
     const float most = fminf(6.0f * unit, __uint_as_float(0x7f400000u));
-    float y[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) y[j] = __builtin_amdgcn_fmed3f(x[j], -most, most);
-    uint32_t code = 0;
-    code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, y[0], y[1], unit, 0);
-    code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, y[2], y[3], unit, 1);
-    code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, y[4], y[5], unit, 2);
-    code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, y[6], y[7], unit, 3);
-    if (!finite) code = 0;
-    const uint32_t slot = a.slots[token];
     const uint32_t page = slot >> a.c.shift, t = slot & (a.c.page - 1u);
-    if (page >= a.c.num_pages) return;
     uint8_t* base = a.cache + (uint64_t)page * a.c.page_bytes + (uint64_t)head * a.c.head_bytes;
-    *reinterpret_cast<uint32_t*>(base + (which ? q4_v_code(a.c, t, chunk) : q4_k_code(a.c, t, chunk))) = code;
-    if ((chunk & 3u) == 0)
-        base[which ? q4_v_scale(a.c, t, chunk >> 2) : q4_k_scale(a.c, t, chunk >> 2)] =
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        float y[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) y[j] = __builtin_amdgcn_fmed3f(x[4 * h + j], -most, most);
+        uint32_t code = 0;
+        code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, y[0], y[1], unit, 0);
+        code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, y[2], y[3], unit, 1);
+        if (!finite) code = 0;
+        const uint32_t chunk = 4 * block + 2 * h + (q >> 1);
+        if (page < a.c.num_pages)
+            *reinterpret_cast<uint16_t*>(base + (which ? q4_v_code(a.c, t, chunk) : q4_k_code(a.c, t, chunk)) + 2 * (q & 1u)) =
+                (uint16_t)code;
+    }
+    if (q == 0 && page < a.c.num_pages)
+        base[which ? q4_v_scale(a.c, t, block) : q4_k_scale(a.c, t, block)] =
             (uint8_t)(finite ? (uint32_t)(e + 127) : kQ4NanScale);
 }
 
-// A lane has dimensions 4q .. 4q + 3 and 16 + 4q .. of its block, q its place among the
-// block's four lanes: each of its two stores and its neighbours' are 64 bytes on end.
 __global__ __launch_bounds__(kQ4Block) void q4_read_kernel(Q4Args a) {
     const uint32_t i = blockIdx.x * kQ4Block + threadIdx.x;
     const int which = blockIdx.y;
     if (i >= a.items) return;
     uint64_t token;
-    uint32_t head, at;
-    q4_item(a, i, &token, &head, &at);
-    const uint32_t block = at >> 2, q = at & 3u;
+    uint32_t head, lane;
+    q4_item(a, i, &token, &head, &lane);
+    const uint32_t block = lane >> 2, q = lane & 3u;
     const uint32_t slot = a.slots[token];
     const uint32_t page = slot >> a.c.shift, t = slot & (a.c.page - 1u);
     uint32_t code[2] = {0, 0}, b = 127;
@@ -148,7 +149,7 @@ __global__ __launch_bounds__(kQ4Block) void q4_read_kernel(Q4Args a) {
         const auto hi = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(code[h], 1.0f, 1);
         const f32x4 v = {lo[0] * s, lo[1] * s, hi[0] * s, hi[1] * s};
         if (d + 4u <= a.head_dim) {
-            *reinterpret_cast<f32x4_a4*>(row + d) = (f32x4_a4)v;
+            __builtin_nontemporal_store((f32x4_a4)v, reinterpret_cast<f32x4_a4*>(row + d));
         } else {
 #pragma unroll
             for (int j = 0; j < 4; ++j)
