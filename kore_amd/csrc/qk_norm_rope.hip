@@ -82,8 +82,20 @@ __device__ __forceinline__ float group_sum(float v) {
     return v;
 }
 
-__device__ __forceinline__ f32x4 ld4(const float* p) { return (f32x4)__builtin_nontemporal_load(reinterpret_cast<const f32x4_a4*>(p)); }
-__device__ __forceinline__ f32x4 ld4_cached(const float* p) { return (f32x4)*reinterpret_cast<const f32x4_a4*>(p); }
+// Rows are read past the caches (kPast) only where they do not fit the last one (256
+// MB): up to 184 MB in and out the caches give 10 % (backward, 4000 x 24 heads of 96:
+// 23.3 -> 20.7 us; forward, 4096 x 40 heads of 128: 28.4 -> 25.4), at 336 MB they cost
+// 4 % (54.0 -> 56.4), at 1007 MB 8 % (171 -> 184).  Results always go past them (through
+// them 12.3 us where 11.2).
+constexpr uint64_t kQkCached = 192ull << 20;
+
+template <bool kPast>
+__device__ __forceinline__ f32x4 ld4(const float* p) {
+    const f32x4_a4* q = reinterpret_cast<const f32x4_a4*>(p);
+    if constexpr (kPast) return (f32x4)__builtin_nontemporal_load(q);
+    return (f32x4)*q;
+}
+__device__ __forceinline__ f32x4 ld4_cached(const float* p) { return ld4<false>(p); }
 __device__ __forceinline__ void st4(float* p, f32x4 v) { __builtin_nontemporal_store((f32x4_a4)v, reinterpret_cast<f32x4_a4*>(p)); }
 
 // The lane's four (cos, sin): half-split pairs 4l .. 4l + 3; interleaved
@@ -119,7 +131,7 @@ __device__ __forceinline__ float dot4(f32x4 a, f32x4 b) {
 
 // One workgroup: 128 / LPR rows of one token's Q or K.  The row's loads are
 // issued first; the token's cos/sin are computed while they are in flight.
-template <int LPR, bool Interleaved>
+template <int LPR, bool Interleaved, bool kPast>
 __global__ __launch_bounds__(kQkBlock) void qk_norm_rope_kernel(QkArgs a) {
     constexpr int kRows = kQkBlock / LPR;
     __shared__ float2 cs[LPR * 4];
@@ -133,8 +145,8 @@ __global__ __launch_bounds__(kQkBlock) void qk_norm_rope_kernel(QkArgs a) {
     f32x4 x0 = {0.f, 0.f, 0.f, 0.f}, x1 = x0, w0 = x0, w1 = x0;
     if (ok) {
         const float* p = a.x[t] + token * a.xs[t] + (uint64_t)row * a.dim + 4 * l;
-        x0 = ld4(p);
-        x1 = ld4(p + half);
+        x0 = ld4<kPast>(p);
+        x1 = ld4<kPast>(p + half);
         w0 = ld4_cached(a.w[t] + 4 * l);
         w1 = ld4_cached(a.w[t] + half + 4 * l);
     }
@@ -185,7 +197,7 @@ __global__ __launch_bounds__(kQkBwBlock) void qk_norm_rope_any_kernel(QkArgs a) 
 // cos/sin are computed for it meanwhile.  Each lane keeps the dw of its eight
 // dimensions over all its rows; the groups' sums meet in LDS at the end and leave as
 // one partial row a workgroup.  Whole: all lanes of a group hold values (D = 8 LPR).
-template <int LPR, bool Interleaved, bool Whole>
+template <int LPR, bool Interleaved, bool Whole, bool kPast>
 __global__ __launch_bounds__(kQkBwBlock) void qk_norm_rope_bwd_kernel(QkArgs a) {
     constexpr uint32_t kGroups = kQkBwBlock / LPR;
     extern __shared__ f32x4 qk_lds[];  // cos/sin [2][span][D / 2], later sums [groups][D]
@@ -210,10 +222,10 @@ __global__ __launch_bounds__(kQkBwBlock) void qk_norm_rope_bwd_kernel(QkArgs a) 
         const uint32_t tok = r / heads, row = r - tok * heads;
         const float* p = x + tok * xs + (uint64_t)row * a.dim + 4 * l;
         const float* d = dy + tok * dys + (uint64_t)row * a.dim + 4 * l;
-        o[0] = ld4(p);
-        o[1] = ld4(p + half);
-        o[2] = ld4(d);
-        o[3] = ld4(d + half);
+        o[0] = ld4<kPast>(p);
+        o[1] = ld4<kPast>(p + half);
+        o[2] = ld4<kPast>(d);
+        o[3] = ld4<kPast>(d + half);
     };
     auto angles = [&](uint32_t run, float2* to) {
         if (run >= rows) return;
@@ -523,6 +535,7 @@ extern "C" int kore_hip_qk_norm_rope_f32(const float* q, const float* k, const f
     if (qk_alias(a, a.x, a.xs, true) || qk_outputs_alias(a) || qk_meets(a, {})) return KORE_HIP_ERR_ALIAS;
     hipStream_t s = (hipStream_t)stream;
     const bool vec = qk_vector(head_dim);
+    const bool past = a.tokens * ((uint64_t)q_heads + k_heads) * head_dim * 8 > kQkCached;
     const uint32_t lanes = qk_lanes(head_dim), rows = kQkBlock / std::min(lanes, 64u);
     a.chunks[0] = (q_heads + rows - 1) / rows;
     a.chunks[1] = (k_heads + rows - 1) / rows;
@@ -535,8 +548,10 @@ extern "C" int kore_hip_qk_norm_rope_f32(const float* q, const float* k, const f
         if (vec) {
             const dim3 grid((uint32_t)(a.tokens * (a.chunks[0] + a.chunks[1])));
 #define QK_CALL(L)                                                                                                     \
-    if (interleaved) hipLaunchKernelGGL((qk_norm_rope_kernel<L, true>), grid, dim3(kQkBlock), 0, s, a);                \
-    else hipLaunchKernelGGL((qk_norm_rope_kernel<L, false>), grid, dim3(kQkBlock), 0, s, a);
+    if (interleaved && past) hipLaunchKernelGGL((qk_norm_rope_kernel<L, true, true>), grid, dim3(kQkBlock), 0, s, a);  \
+    else if (interleaved) hipLaunchKernelGGL((qk_norm_rope_kernel<L, true, false>), grid, dim3(kQkBlock), 0, s, a);    \
+    else if (past) hipLaunchKernelGGL((qk_norm_rope_kernel<L, false, true>), grid, dim3(kQkBlock), 0, s, a);           \
+    else hipLaunchKernelGGL((qk_norm_rope_kernel<L, false, false>), grid, dim3(kQkBlock), 0, s, a);
             QK_LANES(lanes, QK_CALL)
 #undef QK_CALL
         } else {
@@ -620,19 +635,24 @@ extern "C" int kore_hip_qk_norm_rope_backward_f32(
         if (q_heads && k_heads && qk_rows_meet(grad_q_weight, head_dim, head_dim, 1, grad_k_weight, dw))
             return KORE_HIP_ERR_ALIAS;
         const dim3 grid(plan.parts[0] + plan.parts[1]), block(kQkBwBlock);
+        const bool past = a.tokens * ((uint64_t)q_heads + k_heads) * head_dim * 12 > kQkCached;
         if (qk_vector(head_dim)) {
             const uint32_t lanes = qk_lanes(head_dim);
             const uint32_t fewest = !q_heads ? k_heads : !k_heads ? q_heads : std::min(q_heads, k_heads);
             a.span = (plan.groups - 1) / fewest + 2;
             const size_t lds = (size_t)std::max(2 * a.span, plan.groups) * head_dim * sizeof(float);
             const bool whole = head_dim == 8 * lanes;
-#define QK_CALL(L)                                                                                                       \
-    if (interleaved && whole) hipLaunchKernelGGL((qk_norm_rope_bwd_kernel<L, true, true>), grid, block, lds, s, a);      \
-    else if (interleaved) hipLaunchKernelGGL((qk_norm_rope_bwd_kernel<L, true, false>), grid, block, lds, s, a);         \
-    else if (whole) hipLaunchKernelGGL((qk_norm_rope_bwd_kernel<L, false, true>), grid, block, lds, s, a);               \
-    else hipLaunchKernelGGL((qk_norm_rope_bwd_kernel<L, false, false>), grid, block, lds, s, a);
+#define QK_FORM(L, I, W)                                                                                               \
+    if (past) hipLaunchKernelGGL((qk_norm_rope_bwd_kernel<L, I, W, true>), grid, block, lds, s, a);                    \
+    else hipLaunchKernelGGL((qk_norm_rope_bwd_kernel<L, I, W, false>), grid, block, lds, s, a);
+#define QK_CALL(L)                                                                                                     \
+    if (interleaved && whole) { QK_FORM(L, true, true) }                                                               \
+    else if (interleaved) { QK_FORM(L, true, false) }                                                                  \
+    else if (whole) { QK_FORM(L, false, true) }                                                                        \
+    else { QK_FORM(L, false, false) }
             QK_LANES(lanes, QK_CALL)
 #undef QK_CALL
+#undef QK_FORM
         } else {
             const size_t lds = (size_t)(kQkBwBlock / kWave) * head_dim * sizeof(float);
             if (interleaved) hipLaunchKernelGGL(qk_norm_rope_bwd_any_kernel<true>, grid, block, lds, s, a);

@@ -224,3 +224,38 @@ def test_two_backward_calls_at_once():
         torch.cuda.synchronize()
         for g, x in zip(got, want):
             assert all(torch.equal(b.tensor()[:y.numel()], y) for b, y in zip(g, x))
+
+
+@pytest.mark.parametrize("d,inter", [(96, False), (128, True)])
+def test_more_than_the_caches_hold(d, inter):
+    """Rows that are read past the caches: the same bits as from small calls on some of the tokens, and dw in 64 bits."""
+    t, hq, hk = 7000, 32, 8
+    gen = torch.Generator(device="cuda").manual_seed(50)
+    q, k, dq, dk = (torch.randn(t, h, d, device="cuda", generator=gen) for h in (hq, hk, hq, hk))
+    qw, kw, inv = normal((d,), 51, 1.0, 0.1), normal((d,), 52, 1.0, 0.1), rocm.rope_inv_freq_host(d, 10000.0)
+    pos = np.random.default_rng(53).integers(0, 100000, t).astype(np.uint32)
+    w = (up(qw), up(kw), up(inv))
+
+    def call(lo, hi):
+        b = [HipBuffer.from_tensor(x[lo:hi].contiguous()) for x in (q, k, dq, dk)]
+        n = hi - lo
+        y = rocm.rocm_qk_norm_rope_f32(DEV, b[0], b[1], *w, n, 1, hq, hk, d, EPS, 0, up(pos[lo:hi]), inter)
+        g = rocm.rocm_qk_norm_rope_backward_f32(DEV, b[2], b[3], b[0], b[1], *w, n, 1, hq, hk, d, EPS, 0, up(pos[lo:hi]), inter)
+        torch.cuda.synchronize()
+        return [x.tensor(torch.float32) for x in (*y, *g)]
+
+    big = call(0, t)
+    for lo, hi in ((0, 50), (3333, 3400), (t - 31, t)):
+        for i, (a, b) in enumerate(zip(big[:4], call(lo, hi)[:4])):
+            row = (hq, hk)[i % 2] * d
+            assert torch.equal(a[lo * row:hi * row], b[:(hi - lo) * row]), (i, lo)
+    angle = torch.from_numpy(pos.astype(np.float64)).cuda()[:, None] * torch.from_numpy(inv.astype(np.float64)).cuda()
+    c, s = angle.cos()[:, None], angle.sin()[:, None]
+    for i, (x, dy) in enumerate(((q, dq), (k, dk))):
+        x, dy = x.double(), dy.double()
+        a, b = (dy[..., 0::2], dy[..., 1::2]) if inter else (dy[..., :d // 2], dy[..., d // 2:])
+        g0, g1, both = a * c + b * s, b * c - a * s, a.abs() + b.abs()
+        g, size = (torch.stack(p, -1).flatten(-2) if inter else torch.cat(p, -1) for p in ((g0, g1), (both, both)))
+        n = x / ((x * x).mean(-1, keepdim=True) + EPS).sqrt()
+        want, tol = (g * n).sum((0, 1)), ((192 + 64) * q4_ref.U + 3 * 2.0 ** -53 * 1e5) * (size * n.abs()).sum((0, 1))
+        assert ((big[4 + i][:d].double() - want).abs() <= tol).all()
